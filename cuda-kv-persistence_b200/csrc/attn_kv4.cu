@@ -1,0 +1,414 @@
+// Attention over the 4-bit K/V cache (kv4.h): the kernel for few query rows
+// and the launcher.
+//
+// For query row i of sequence b at position p = start + i in frame f = p / T,
+//   out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),
+//   x_j = q . k_j * log2(e) / sqrt(128),
+// over the keys j < min((f + 1) T, start + count) with j >= max(f - W + 1, 0) T
+// (W = 0: every j) or j < S T.  No visible key: 0.  The query rows of a K/V
+// head are its (row, query head of the group) pairs, row fastest-changing
+// last: r = i * group + g.
+#include <algorithm>
+#include <cstring>
+
+#include "attn_kv4.cuh"
+#include "kernels.h"
+#include "kv4.h"
+
+namespace kvp {
+
+namespace {
+
+using namespace kv4_dev;
+
+// ------------------------------------------------- few query rows: mma.sync
+// Bound by the cache's bytes: 144 a key and K/V head, against 2 * 128 * 2
+// multiply-adds per query row.  Keys and dims go on the M side of
+// m16n8k16 and the query rows on the N side, so up to 8 rows cost the same:
+//   S^T[16 keys x 8] = K[16 x 128] Q^T,  O^T[16 dims x 8] += V^T[16 x 16] P^T.
+// A lane's fragment of K is one 16-byte word of a row (a quarter of its dims;
+// the order of the dims inside the sum is free, Q's fragment follows it), its
+// fragment of V is two neighbouring rows of one 16-dim group, so both come
+// straight from global memory, 512 consecutive bytes a warp, without shared
+// memory; movmatrix turns P^T into the second product's operand.
+constexpr int kWarps = 8;
+constexpr int kDecThreads = kWarps * 32;
+constexpr int kKeys = 16;                      // keys of one step of a warp
+constexpr float kRise = 8.f;                   // log2: how far a score may pass the running max
+
+struct Step {
+    uint4 k0, k1, v0, v1;                      // K / V codes of the two 8-row blocks
+    uint32_t ks, vs;                           // their scale bytes, block 0 low
+    int key;                                   // first key position
+    bool bad;                                  // the page is not in the pool
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return reinterpret_cast<const uint32_t&>(h);
+}
+
+template <int NB>
+struct RowsSmem {
+    float o[kWarps][8 * NB][kKv4Head];
+    float m[kWarps][8 * NB], l[kWarps][8 * NB];
+};
+
+// NB blocks of 8 query rows.
+template <int NB>
+__global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_kernel(const Kv4Params P) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    RowsSmem<NB>& sm = *reinterpret_cast<RowsSmem<NB>*>(smem_raw);
+    const Kv4Span& s = P.span;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    // CTA = (split, row tile, K/V head, sequence), split fastest
+    long long x = blockIdx.x;
+    const int split = (int)(x % P.splits);
+    x /= P.splits;
+    const int tile = (int)(x % P.row_tiles);
+    x /= P.row_tiles;
+    const int h = (int)(x % s.kv_heads), b = (int)(x / s.kv_heads);
+    int start, count;
+    if (!sequence(s, b, start, count)) {
+        if (threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_MAP);
+        return;
+    }
+    const int rows = count * P.group, r0 = tile * 8 * NB;
+    if (r0 >= rows) return;
+    const int end = start + count;
+    const Sees first = sees(P, start + r0 / P.group, end);
+    const Sees last = sees(P, start + (min(r0 + 8 * NB, rows) - 1) / P.group, end);
+    // 16-key steps: those of the sinks below the window, then the window's
+    const int b0 = first.lo / kKeys, nb = (last.hi + kKeys - 1) / kKeys - b0;
+    const int na = min((min(P.sink_rows, last.hi) + kKeys - 1) / kKeys, b0);
+    const int n = na + nb, per = (n + P.splits - 1) / P.splits;
+    const int u0 = min(split * per, n), u1 = min(u0 + per, n);
+
+    // Q^T fragments: step 2w + j of the 128 dims is dims 32t + 8w + 4j .. + 3
+    uint32_t qf[NB][16];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int r = r0 + 8 * i + g;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint4 y = make_uint4(0, 0, 0, 0);
+            if (r < rows)
+                y = __ldg(reinterpret_cast<const uint4*>(q_row(P, b, h, r) + 32 * t + 8 * w));
+            qf[i][4 * w] = y.x; qf[i][4 * w + 1] = y.y; qf[i][4 * w + 2] = y.z; qf[i][4 * w + 3] = y.w;
+        }
+    }
+    // the rows of this lane's two score columns
+    int hi[NB][2], lo[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int r = min(r0 + 8 * i + 2 * t + c, rows - 1);
+            const Sees e = sees(P, start + r / P.group, end);
+            hi[i][c] = e.hi;
+            lo[i][c] = e.lo;
+        }
+    float m[NB][2], l[NB][2], o[NB][8][4];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        m[i][0] = m[i][1] = -INFINITY;
+        l[i][0] = l[i][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+    }
+
+    auto key_of = [&](int u) { return (u < na ? u : u - na + b0) * kKeys; };
+    auto lookup = [&](int u) { return u < u1 ? page_of(s, b, key_of(u) / kKv4PageRows) : 0; };
+    auto load = [&](int u, int page) {
+        Step z;
+        z.key = key_of(u);
+        z.bad = page < 0;
+        const uint8_t* p = static_cast<const uint8_t*>(s.pages) +
+                           ((long long)(page < 0 ? 0 : page) * s.kv_heads + h) * kKv4PageHeadBytes +
+                           (z.key % kKv4PageRows) / kKv4BlockRows * kKv4BlockBytes;
+        z.k0 = *reinterpret_cast<const uint4*>(p + lane * 16);
+        z.k1 = *reinterpret_cast<const uint4*>(p + kKv4BlockBytes + lane * 16);
+        z.v0 = *reinterpret_cast<const uint4*>(p + kKv4VCode + lane * 16);
+        z.v1 = *reinterpret_cast<const uint4*>(p + kKv4BlockBytes + kKv4VCode + lane * 16);
+        z.ks = *reinterpret_cast<const uint16_t*>(p + kKv4KScale + lane * 2) |
+               (uint32_t)*reinterpret_cast<const uint16_t*>(p + kKv4BlockBytes + kKv4KScale + lane * 2) << 16;
+        z.vs = *reinterpret_cast<const uint16_t*>(p + kKv4VScale + lane * 2) |
+               (uint32_t)*reinterpret_cast<const uint16_t*>(p + kKv4BlockBytes + kKv4VScale + lane * 2) << 16;
+        return z;
+    };
+    auto compute = [&](const Step& z) {
+        // S^T
+        float c[NB][4];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+        const uint32_t k0[4] = {z.k0.x, z.k0.y, z.k0.z, z.k0.w}, k1[4] = {z.k1.x, z.k1.y, z.k1.z, z.k1.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            // words 0, 1 are the quarter's first 16-dim group, 2, 3 the second
+            const Scale2 s0 = scale2(__byte_perm(z.ks, 0, w < 2 ? 0x4040 : 0x4141));
+            const Scale2 s1 = scale2(__byte_perm(z.ks, 0, w < 2 ? 0x4242 : 0x4343));
+            const uint32_t a0 = field<0>(k0[w], s0), a1 = field<0>(k1[w], s1);
+            const uint32_t a2 = field<1>(k0[w], s0), a3 = field<1>(k1[w], s1);
+            const uint32_t a4 = field<2>(k0[w], s0), a5 = field<2>(k1[w], s1);
+            const uint32_t a6 = field<3>(k0[w], s0), a7 = field<3>(k1[w], s1);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                mma16816(c[i], a0, a1, a2, a3, qf[i][4 * w], qf[i][4 * w + 1]);
+                mma16816(c[i], a4, a5, a6, a7, qf[i][4 * w + 2], qf[i][4 * w + 3]);
+            }
+        }
+        // masks, running max, P
+        const bool whole = !z.bad && z.key + kKeys <= first.hi &&
+                           (z.key >= last.lo || z.key + kKeys <= P.sink_rows);
+        bool rise = false;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = z.key + g + 8 * (e >> 1);
+                c[i][e] *= P.scale_log2;
+                if (!whole && (z.bad || key >= hi[i][e & 1] || (key < lo[i][e & 1] && key >= P.sink_rows)))
+                    c[i][e] = -INFINITY;
+                rise |= c[i][e] > m[i][e & 1] + kRise;
+            }
+        // The max moves only when some score passes it by more than 2^8 (or a
+        // row sees its first key): P then stays below 2^8, far inside fp32 and
+        // bf16, and most steps need no reduction over the keys.
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    float top = fmaxf(c[i][a], c[i][a + 2]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float up = fmaxf(m[i][a], top);
+                    const float f = up == m[i][a] ? 1.f : ex2(m[i][a] - up);
+                    m[i][a] = up;
+                    l[i][a] *= f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        o[i][j][a] *= f;
+                        o[i][j][a + 2] *= f;
+                    }
+                }
+        }
+        uint32_t p0[NB], p1[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const float ma = m[i][0] == -INFINITY ? 0.f : m[i][0], mb = m[i][1] == -INFINITY ? 0.f : m[i][1];
+            const float e0 = ex2(c[i][0] - ma), e1 = ex2(c[i][1] - mb);
+            const float e2 = ex2(c[i][2] - ma), e3 = ex2(c[i][3] - mb);
+            l[i][0] += e0 + e2;
+            l[i][1] += e1 + e3;
+            // P to bf16 (a tensor-core operand): half a step, 2^-9 of each
+            // weight, without bias; the sum l keeps 32 bits
+            p0[i] = transpose8(pack2(e0, e1));
+            p1[i] = transpose8(pack2(e2, e3));
+        }
+        // O^T: word d of a row holds dims 16g + 8d + 2i (low half's field i)
+        // and + 1 (high half's); pairing two rows' halves puts two keys of one
+        // dim into a register
+        const Scale2 s0 = scale2(__byte_perm(z.vs, 0, 0x4140)), s1 = scale2(__byte_perm(z.vs, 0, 0x4342));
+        const uint32_t va[2] = {z.v0.x, z.v0.y}, vb[2] = {z.v0.z, z.v0.w};
+        const uint32_t vc[2] = {z.v1.x, z.v1.y}, vd[2] = {z.v1.z, z.v1.w};
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            const uint32_t e0 = __byte_perm(va[d], vb[d], 0x5410), o0 = __byte_perm(va[d], vb[d], 0x7632);
+            const uint32_t e1 = __byte_perm(vc[d], vd[d], 0x5410), o1 = __byte_perm(vc[d], vd[d], 0x7632);
+            auto step = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) mma16816(o[i][j], a0, a1, a2, a3, p0[i], p1[i]);
+            };
+            step(4 * d, field<0>(e0, s0), field<0>(o0, s0), field<0>(e1, s1), field<0>(o1, s1));
+            step(4 * d + 1, field<1>(e0, s0), field<1>(o0, s0), field<1>(e1, s1), field<1>(o1, s1));
+            step(4 * d + 2, field<2>(e0, s0), field<2>(o0, s0), field<2>(e1, s1), field<2>(o1, s1));
+            step(4 * d + 3, field<3>(e0, s0), field<3>(o0, s0), field<3>(e1, s1), field<3>(o1, s1));
+        }
+    };
+
+    // A warp takes every eighth step of the CTA's range; the next step's bytes
+    // and the page number after that are in flight while one is computed.
+    bool bad = false;
+    int u = u0 + warp;
+    if (u < u1) {
+        Step cur = load(u, lookup(u));
+        int page = lookup(u + kWarps);
+        for (; u < u1; u += kWarps) {
+            Step nxt = cur;
+            if (u + kWarps < u1) nxt = load(u + kWarps, page);
+            page = lookup(u + 2 * kWarps);
+            bad |= cur.bad;
+            compute(cur);
+            cur = nxt;
+        }
+    }
+    if (bad && lane == 0) atomicOr(P.status, KVP_STATUS_MAP);
+
+    // Join the warps: l over the lanes of a column, then (O, m, l) over the warps.
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            l[i][a] += __shfl_xor_sync(0xffffffffu, l[i][a], 4);
+            l[i][a] += __shfl_xor_sync(0xffffffffu, l[i][a], 8);
+            l[i][a] += __shfl_xor_sync(0xffffffffu, l[i][a], 16);
+            const int q = 8 * i + 2 * t + a;
+            if (g == 0) {
+                sm.m[warp][q] = m[i][a];
+                sm.l[warp][q] = l[i][a];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                *reinterpret_cast<float4*>(&sm.o[warp][q][16 * g + 2 * j]) =
+                    make_float4(o[i][j][a], o[i][j][a + 2], o[i][j + 1][a], o[i][j + 1][a + 2]);
+        }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 8 * NB * (kKv4Head / 4); e += kDecThreads) {
+        const int q = e / (kKv4Head / 4), d = e % (kKv4Head / 4) * 4;
+        const int r = r0 + q;
+        if (r >= rows) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.m[w][q]);
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (sm.l[w][q] == 0.f) continue;            // no key of this row
+            const float f = ex2(sm.m[w][q] - top);
+            sum += f * sm.l[w][q];
+            const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][q][d]);
+            acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
+        }
+        put(P, b, h, r, split, d, acc, top, sum);
+    }
+}
+
+// ------------------------------------------------------------- joining splits
+// One warp per (sequence, K/V head, row), four dims a lane.
+__global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
+    const Kv4Span& s = P.span;
+    const int lane = threadIdx.x & 31;
+    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (w >= (long long)s.batch * s.kv_heads * P.max_rows) return;
+    const int r = (int)(w % P.max_rows);
+    const int h = (int)(w / P.max_rows % s.kv_heads), b = (int)(w / P.max_rows / s.kv_heads);
+    int start, count;
+    if (!sequence(s, b, start, count) || r >= count * P.group) return;
+    const float2* ml = reinterpret_cast<const float2*>(P.ws_ml) + w * P.splits;
+    float top = -INFINITY;
+    for (int c = 0; c < P.splits; ++c) top = fmaxf(top, ml[c].x);
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < P.splits; ++c) {
+        const float2 y = ml[c];
+        if (y.y == 0.f) continue;                     // no key of this row
+        const float f = ex2(y.x - top);
+        sum += f * y.y;
+        const float4 o = reinterpret_cast<const float4*>(P.ws_o + (w * P.splits + c) * kKv4Head)[lane];
+        acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
+    }
+    store_out(P, b, h, r, 4 * lane, acc, sum);
+}
+
+template <int NB>
+int launch_rows(const Kv4Params& P, unsigned grid, cudaStream_t stream) {
+    static PerDeviceOnce setup;
+    const int rc = setup([](int) -> int {
+        KVP_CUDA(cudaFuncSetAttribute(attn_kv4_rows_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)sizeof(RowsSmem<NB>)));
+        return KVP_OK;
+    });
+    if (rc != KVP_OK) return rc;
+    attn_kv4_rows_kernel<NB><<<grid, kDecThreads, sizeof(RowsSmem<NB>), stream>>>(P);
+    KVP_CUDA(cudaGetLastError());
+    return KVP_OK;
+}
+
+int sm_count() {
+    int n = 148, dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n > 0 ? n : 148;
+}
+
+}  // namespace
+
+int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStream_t stream) {
+    const int rc = check_kv4_attn(s, a);
+    if (rc != KVP_OK || s.rows == 0 || s.batch == 0) return rc;
+    Kv4Params P;
+    std::memset(&P, 0, sizeof P);
+    P.span = s;
+    P.attn = a;
+    P.status = d_status;
+    P.group = a.heads / s.kv_heads;
+    P.max_rows = s.rows * P.group;
+    const long long cap = (long long)s.map_stride * kKv4PageRows;
+    // beyond the capacity a window or a sink hides nothing and a frame is all
+    P.tokens = a.tokens;
+    P.window_rows = a.window ? std::min<long long>((long long)a.window * a.tokens, 1LL << 31) : 0;
+    P.sink_rows = (int)std::min<long long>((long long)a.sinks * a.tokens, cap);
+    P.scale_log2 = 1.4426950408889634f / sqrtf((float)kKv4Head);
+
+    const int nb = P.max_rows > 8 ? 2 : 1;
+    P.row_tiles = (P.max_rows + 8 * nb - 1) / (8 * nb);
+    const long long units = (long long)s.batch * s.kv_heads * P.row_tiles;
+    // Key steps of a row tile, at most (starts on the device: the capacity's).
+    long long keys = s.starts ? cap : (long long)s.start + s.rows;
+    if (a.window) {
+        const long long span = (long long)(8 * nb / P.group + 2 + a.tokens) + (long long)P.window_rows + P.sink_rows + 32;
+        keys = std::min(keys, span);
+    }
+    // Two CTAs an SM; a split keeps a step for each warp.
+    const long long want = (2LL * sm_count() + units - 1) / units;
+    const long long most = (keys + kKeys * kWarps - 1) / (kKeys * kWarps);
+    P.splits = (int)std::max<long long>(1, std::min(std::min(want, most), 256LL));
+    const long long grid = units * P.splits;
+    if (grid > 0x7fffffffLL) {
+        set_error("attn_kv4: too many rows for one launch");
+        return KVP_ERR_ARG;
+    }
+    const long long slots = (long long)s.batch * s.kv_heads * P.max_rows * P.splits;
+    void* ws = nullptr;
+    if (P.splits > 1) {
+        cudaMemPool_t pool = nullptr;
+        KVP_CUDA(workspace_pool(&pool));
+        KVP_CUDA(cudaMallocFromPoolAsync(&ws, (size_t)slots * (kKv4Head + 2) * sizeof(float), pool, stream));
+        P.ws_o = static_cast<float*>(ws);
+        P.ws_ml = P.ws_o + slots * kKv4Head;
+    }
+    int launched = nb == 1 ? launch_rows<1>(P, (unsigned)grid, stream) : launch_rows<2>(P, (unsigned)grid, stream);
+    if (ws) {
+        if (launched == KVP_OK) {
+            const long long warps = slots / P.splits;
+            attn_kv4_join_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(P);
+            const cudaError_t e = cudaGetLastError();
+            if (e != cudaSuccess) launched = cuda_status(e, "attn_kv4 join");
+        }
+        const cudaError_t e = cudaFreeAsync(ws, stream);
+        if (e != cudaSuccess && launched == KVP_OK) launched = cuda_status(e, "attn_kv4 workspace");
+    }
+    return launched;
+}
+
+}  // namespace kvp

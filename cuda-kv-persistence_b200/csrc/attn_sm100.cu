@@ -935,6 +935,8 @@ combine_splits_kernel(const float* __restrict__ ws, __nv_bfloat16* __restrict__ 
     *reinterpret_cast<uint2*>(out + (size_t)(row0 + rr) * D + (size_t)(head0 + h) * kDH + 4 * lane) = pk;
 }
 
+}  // namespace
+
 // The split workspace comes from a private, per-device stream-ordered pool
 // that keeps freed blocks cached (release threshold = max): the default
 // pool would hand its memory back to the driver at every synchronisation
@@ -966,6 +968,8 @@ cudaError_t workspace_pool(cudaMemPool_t* out) {
     *out = pools[dev];
     return cudaSuccess;
 }
+
+namespace {
 
 // Key chunks per (query tile pair, head) for a per-frame launch: split only
 // when the launch has fewer CTAs than SMs; minimise waves x (fixed cost +

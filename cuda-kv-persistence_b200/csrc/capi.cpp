@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "kv4.h"
 #include "kv_tile_manager.h"
 #include "kvp_common.h"
 #include "motion_sm100.h"
@@ -724,4 +725,76 @@ KVP_API int kvp_session_run_frames_batched(void* sp, int f0, int nframes, const 
         if (rc != kvp::KVP_OK) return rc;
     }
     return persist ? s->clear_window(st) : kvp::KVP_OK;
+}
+
+// ----------------------------------------------------------- 4-bit K/V cache
+// Field meanings: include/kvp.h.  Nothing here reads what the kvtm_*
+// managers stage, so their queued copies are left alone.
+struct kvp_kv4_span {
+    void* pages;
+    const int* page_map;
+    const int* starts;
+    const int* counts;
+    long long n_pages;
+    int kv_heads, batch, map_stride, start, rows;
+};
+
+struct kvp_kv4_rows {
+    void* k;
+    void* v;
+    long long row_stride, batch_stride;
+    int elem_bytes;
+};
+
+struct kvp_kv4_attn {
+    const void* q;
+    void* out;
+    long long q_row_stride, q_batch_stride, out_row_stride, out_batch_stride;
+    int heads, tokens, window, sinks;
+};
+
+namespace {
+kvp::Kv4Span span_of(const kvp_kv4_span& s) {
+    return kvp::Kv4Span{s.pages, s.page_map, s.starts, s.counts, s.n_pages,
+                        s.kv_heads, s.batch, s.map_stride, s.start, s.rows};
+}
+}  // namespace
+
+KVP_API long long kvp_kv4_page_bytes(int kv_heads) {
+    return kv_heads > 0 ? (long long)kv_heads * kvp::kKv4PageHeadBytes : kvp::KVP_ERR_ARG;
+}
+
+KVP_API int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream) {
+    if (!s || !r) return kvp::KVP_ERR_ARG;
+    const kvp::Kv4Span S = span_of(*s);
+    const kvp::Kv4Rows R{r->k, r->v, r->row_stride, r->batch_stride, r->elem_bytes};
+    // Bad arguments are reported before any device state is touched.
+    const int rc = kvp::check_kv4_rows(S, R, true);
+    if (rc != kvp::KVP_OK) return rc;
+    int* st = kvp::status_word();
+    if (!st) return kvp::KVP_ERR_CUDA;
+    return kvp::launch_kv4_write(S, R, st, (cudaStream_t)stream);
+}
+
+KVP_API int kvp_kv4_read(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream) {
+    if (!s || !r) return kvp::KVP_ERR_ARG;
+    const kvp::Kv4Span S = span_of(*s);
+    const kvp::Kv4Rows R{r->k, r->v, r->row_stride, r->batch_stride, r->elem_bytes};
+    const int rc = kvp::check_kv4_rows(S, R, false);
+    if (rc != kvp::KVP_OK) return rc;
+    int* st = kvp::status_word();
+    if (!st) return kvp::KVP_ERR_CUDA;
+    return kvp::launch_kv4_read(S, R, st, (cudaStream_t)stream);
+}
+
+KVP_API int kvp_attn_kv4(const kvp_kv4_span* s, const kvp_kv4_attn* a, void* stream) {
+    if (!s || !a) return kvp::KVP_ERR_ARG;
+    const kvp::Kv4Span S = span_of(*s);
+    const kvp::Kv4Attn A{a->q, a->out, a->q_row_stride, a->q_batch_stride, a->out_row_stride,
+                         a->out_batch_stride, a->heads, a->tokens, a->window, a->sinks};
+    const int rc = kvp::check_kv4_attn(S, A);
+    if (rc != kvp::KVP_OK) return rc;
+    int* st = kvp::status_word();
+    if (!st) return kvp::KVP_ERR_CUDA;
+    return kvp::launch_attn_kv4(S, A, st, (cudaStream_t)stream);
 }

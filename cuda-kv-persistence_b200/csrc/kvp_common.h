@@ -25,6 +25,7 @@ enum Status : int {
 constexpr int KVP_STATUS_MAP = 1;      // a KVMap entry pointed outside the arena (base row used)
 constexpr int KVP_STATUS_TIMEOUT = 2;  // a bounded wait expired; the CTA's output is incomplete
 constexpr int KVP_STATUS_ALIGN = 4;    // dynamic shared memory not 1024-byte aligned; nothing computed
+constexpr int KVP_STATUS_RANGE = 8;    // a value the 4-bit cache cannot hold (NaN, or beyond its range) was stored
 
 // The current device's status word (device int, allocated on first use;
 // kvp_read_status reads and clears it).  nullptr if it cannot be allocated.
@@ -43,6 +44,10 @@ const char* last_error();
 // Records the message of CUDA error e and returns KVP_ERR_CUDA (call it
 // only for e != cudaSuccess; KVP_CUDA below does the check).
 int cuda_status(cudaError_t e, const char* what);
+
+// The current device's private stream-ordered pool for split workspaces; it
+// keeps freed blocks cached (attn_sm100.cu).
+cudaError_t workspace_pool(cudaMemPool_t* out);
 
 // Per-device one-time setup (kernel attributes, launch checks): `run` is
 // called under a lock until it succeeds once on the current device; later

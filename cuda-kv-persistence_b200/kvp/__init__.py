@@ -18,3 +18,4 @@ from .layout import TileLayout  # noqa: F401
 from .manager import KVTileManager, KVTM_ADMITTED, KVTM_INVALID, KVTM_REFUSED_BUDGET  # noqa: F401
 from .policies import POLICIES, select  # noqa: F401
 from .session import Session  # noqa: F401
+from . import kv4  # noqa: F401

@@ -66,6 +66,24 @@ class StepInfo(C.Structure):
                 ("restaged", C.c_int), ("hits", C.c_int)]
 
 
+class Kv4Span(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("page_map", C.c_void_p), ("starts", C.c_void_p),
+                ("counts", C.c_void_p), ("n_pages", C.c_longlong), ("kv_heads", C.c_int),
+                ("batch", C.c_int), ("map_stride", C.c_int), ("start", C.c_int), ("rows", C.c_int)]
+
+
+class Kv4Rows(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("row_stride", C.c_longlong),
+                ("batch_stride", C.c_longlong), ("elem_bytes", C.c_int)]
+
+
+class Kv4Attn(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_row_stride", C.c_longlong),
+                ("q_batch_stride", C.c_longlong), ("out_row_stride", C.c_longlong),
+                ("out_batch_stride", C.c_longlong), ("heads", C.c_int), ("tokens", C.c_int),
+                ("window", C.c_int), ("sinks", C.c_int)]
+
+
 # name -> (restype, argtypes); every symbol include/*.h declares.
 SIGNATURES = {
     # include/kv_tile_manager.h
@@ -154,6 +172,10 @@ SIGNATURES = {
                                        C.c_void_p, C.c_void_p]),
     "kvp_layernorm_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_longlong,
                                      C.c_int, C.c_float, C.c_void_p]),
+    "kvp_kv4_page_bytes": (C.c_longlong, [C.c_int]),
+    "kvp_kv4_write": (C.c_int, [C.POINTER(Kv4Span), C.POINTER(Kv4Rows), C.c_void_p]),
+    "kvp_kv4_read": (C.c_int, [C.POINTER(Kv4Span), C.POINTER(Kv4Rows), C.c_void_p]),
+    "kvp_attn_kv4": (C.c_int, [C.POINTER(Kv4Span), C.POINTER(Kv4Attn), C.c_void_p]),
     "kvp_session_plan_stack": (C.c_int, [C.c_void_p, C.c_void_p]),
     "kvp_session_finish": (C.c_int, [C.c_void_p]),
     "kvp_session_info": (C.c_int, [C.c_void_p, C.POINTER(StepInfo)]),

@@ -19,7 +19,8 @@ const char* kvp_last_error(void);
 
 /* Device status word written by the kernels: bit 0 = a KVMap entry pointed
  * outside the arena (the base row was read instead), bit 1 = a bounded
- * device wait expired.  Synchronises `stream`, returns and clears it. */
+ * device wait expired, bit 3 = the 4-bit cache was given a value it cannot
+ * hold (kvp_kv4_write).  Synchronises `stream`, returns and clears it. */
 int kvp_read_status(void* stream);
 
 /* Diagnostics: launches one kernel whose bounded mbarrier wait can never
@@ -297,6 +298,76 @@ int kvp_session_run_frames(void* s, int f0, int nframes, const float* scores_fla
 int kvp_session_run_frames_batched(void* s, int f0, int nframes, const float* scores_flat,
                                    const kvp_layer_io* io, const kvp_attn_desc* d,
                                    long long* maps, void* stream);
+
+/* ---- 4-bit K/V cache and attention over it (no reference counterpart: the
+ * reference keeps K/V in fp32).  144 bytes a row and head for K and V, where
+ * bf16 takes 512.
+ *
+ * The cache is a pool of pages of 128 rows, kvp_kv4_page_bytes(kv_heads)
+ * bytes each, in device memory of the caller; a row is one token's K and V
+ * of every K/V head (128 dims a head).  16 dims share a scale of 4
+ * significant bits, max |x| / 7 rounded to nearest, and hold x / scale
+ * rounded to an integer in [-7, 7], so a value comes back off by at most
+ * half a scale.  A page's bytes may be anything before they are written:
+ * every bit pattern stands for finite numbers.
+ *
+ * A call touches rows [start, start + count) of each of `batch` sequences;
+ * row i of a sequence is position start + i, and its page is
+ * page_map[sequence * map_stride + position / 128].  Page numbers outside
+ * [0, n_pages) set status bit 0: their rows are not written, read back as
+ * zeros, and are no keys.  Pages that no row or query of the call needs are not
+ * looked up.  Two positions of one call's written rows must not share a
+ * page's row.  A sequence whose device start or count does not fit (start <
+ * 0, count not in [0, rows], start + count > 128 * map_stride) sets status
+ * bit 0 and is left alone, its outputs too; so are rows at and behind
+ * its count.  No call allocates for its results or waits for the device;
+ * the buffers belong to the current device. */
+typedef struct {
+    void* pages;
+    const int* page_map;  /* device int32 [batch][map_stride], or NULL: pages sequence * map_stride + p */
+    const int* starts;    /* device int32 [batch], or NULL: `start` for every sequence */
+    const int* counts;    /* device int32 [batch], or NULL: `rows` for every sequence */
+    long long n_pages;
+    int kv_heads, batch;
+    int map_stride;       /* pages a sequence can have; at most 2^30 rows */
+    int start, rows;
+} kvp_kv4_span;
+
+/* K and V rows: head h of row i of sequence b is at element b * batch_stride
+ * + i * row_stride + 128 * h of k and of v (16-byte aligned rows). */
+typedef struct {
+    void* k;
+    void* v;              /* kvp_kv4_read: either may be NULL */
+    long long row_stride, batch_stride;
+    int elem_bytes;       /* 2 = bf16, 4 = fp32 (rounded to bf16 as it is written) */
+} kvp_kv4_rows;
+
+typedef struct {
+    const void* q;        /* bf16, laid out as kvp_kv4_rows with `heads` heads */
+    void* out;            /* bf16, likewise */
+    long long q_row_stride, q_batch_stride, out_row_stride, out_batch_stride;
+    int heads;            /* a multiple of kv_heads; head h reads K/V head h / (heads / kv_heads) */
+    int tokens;           /* rows per frame (1: causal by row) */
+    int window;           /* frames visible, the row's own included; 0 = all (1: intra-frame) */
+    int sinks;            /* first frames that stay visible whatever the window */
+} kvp_kv4_attn;
+
+long long kvp_kv4_page_bytes(int kv_heads);
+
+/* Quantises the rows into the cache.  NaN is stored as 0 and |x| > 860160 as
+ * that bound; either sets status bit 3. */
+int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream);
+
+/* The values the rows stand for (exact in bf16 and fp32). */
+int kvp_kv4_read(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream);
+
+/* softmax(q K^T / sqrt(128)) V over the cache: query row i of a sequence, at
+ * position p = start + i in frame f = p / tokens, sees the positions below
+ * min((f + 1) * tokens, start + count) that are in frames f - window + 1 ..
+ * f or in the first `sinks` frames.  (The call's own rows are keys too: write
+ * them first.)  A row that sees no key is 0.  One row per sequence is a
+ * decoding step, tokens = 1 a causal prompt, tokens = 1560 a video frame. */
+int kvp_attn_kv4(const kvp_kv4_span* s, const kvp_kv4_attn* a, void* stream);
 
 #ifdef __cplusplus
 }
