@@ -33,15 +33,8 @@ using namespace kv4_dev;
 // memory; movmatrix turns P^T into the second product's operand.
 constexpr int kWarps = 8;
 constexpr int kDecThreads = kWarps * 32;
-constexpr int kKeys = 16;                      // keys of one step of a warp
-constexpr float kRise = 8.f;                   // log2: how far a score may pass the running max
-
-struct Step {
-    uint4 k0, k1, v0, v1;                      // K / V codes of the two 8-row blocks
-    uint32_t ks, vs;                           // their scale bytes, block 0 low
-    int key;                                   // first key position
-    bool bad;                                  // the page is not in the pool
-};
+constexpr int kKeys = 32;                      // keys of one step of a warp
+constexpr float kRise = 8.f;                   // how far a score may pass the running max, log2 units
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -87,6 +80,7 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
     x /= P.row_tiles;
     const int h = (int)(x % s.kv_heads), b = (int)(x / s.kv_heads);
     int start, count;
+    cudaTriggerProgrammaticLaunchCompletion();        // the join may be launched; it waits for the data
     if (!sequence(s, b, start, count)) {
         if (threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_MAP);
         return;
@@ -96,7 +90,7 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
     const int end = start + count;
     const Sees first = sees(P, start + r0 / P.group, end);
     const Sees last = sees(P, start + (min(r0 + 8 * NB, rows) - 1) / P.group, end);
-    // 16-key steps: those of the sinks below the window, then the window's
+    // key steps: those of the sinks below the window, then the window's
     const int b0 = first.lo / kKeys, nb = (last.hi + kKeys - 1) / kKeys - b0;
     const int na = min((min(P.sink_rows, last.hi) + kKeys - 1) / kKeys, b0);
     const int n = na + nb, per = (n + P.splits - 1) / P.splits;
@@ -115,18 +109,7 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
             qf[i][4 * w] = y.x; qf[i][4 * w + 1] = y.y; qf[i][4 * w + 2] = y.z; qf[i][4 * w + 3] = y.w;
         }
     }
-    // the rows of this lane's two score columns
-    int hi[NB][2], lo[NB][2];
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int r = min(r0 + 8 * i + 2 * t + c, rows - 1);
-            const Sees e = sees(P, start + r / P.group, end);
-            hi[i][c] = e.hi;
-            lo[i][c] = e.lo;
-        }
-    float m[NB][2], l[NB][2], o[NB][8][4];
+    float m[NB][2], l[NB][2], o[NB][8][4];       // m in score units (before the scale)
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
         m[i][0] = m[i][1] = -INFINITY;
@@ -135,74 +118,115 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
         for (int j = 0; j < 8; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
     }
 
+    const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
+    const uint8_t* head = static_cast<const uint8_t*>(s.pages) + h * kKv4PageHeadBytes;
     auto key_of = [&](int u) { return (u < na ? u : u - na + b0) * kKeys; };
     auto lookup = [&](int u) { return u < u1 ? page_of(s, b, key_of(u) / kKv4PageRows) : 0; };
-    auto load = [&](int u, int page) {
-        Step z;
-        z.key = key_of(u);
-        z.bad = page < 0;
-        const uint8_t* p = static_cast<const uint8_t*>(s.pages) +
-                           ((long long)(page < 0 ? 0 : page) * s.kv_heads + h) * kKv4PageHeadBytes +
-                           (z.key % kKv4PageRows) / kKv4BlockRows * kKv4BlockBytes;
-        z.k0 = *reinterpret_cast<const uint4*>(p + lane * 16);
-        z.k1 = *reinterpret_cast<const uint4*>(p + kKv4BlockBytes + lane * 16);
-        z.v0 = *reinterpret_cast<const uint4*>(p + kKv4VCode + lane * 16);
-        z.v1 = *reinterpret_cast<const uint4*>(p + kKv4BlockBytes + kKv4VCode + lane * 16);
-        z.ks = *reinterpret_cast<const uint16_t*>(p + kKv4KScale + lane * 2) |
-               (uint32_t)*reinterpret_cast<const uint16_t*>(p + kKv4BlockBytes + kKv4KScale + lane * 2) << 16;
-        z.vs = *reinterpret_cast<const uint16_t*>(p + kKv4VScale + lane * 2) |
-               (uint32_t)*reinterpret_cast<const uint16_t*>(p + kKv4BlockBytes + kKv4VScale + lane * 2) << 16;
-        return z;
+    auto at = [&](int u, int page) {
+        return head + (unsigned long long)(uint32_t)max(page, 0) * page_bytes +
+               key_of(u) % kKv4PageRows / kKv4BlockRows * kKv4BlockBytes;
     };
-    auto compute = [&](const Step& z) {
+    uint4 kc[4], vc[4];                            // codes of the step's four 8-row blocks
+    uint32_t ks[4], vs[4];                         // their scale bytes
+    auto load_k = [&](const uint8_t* p) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            kc[j] = *reinterpret_cast<const uint4*>(p + j * kKv4BlockBytes + lane * 16);
+            ks[j] = *reinterpret_cast<const uint16_t*>(p + j * kKv4BlockBytes + kKv4KScale + lane * 2);
+        }
+    };
+    auto load_v = [&](const uint8_t* p) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            vc[j] = *reinterpret_cast<const uint4*>(p + j * kKv4BlockBytes + kKv4VCode + lane * 16);
+            vs[j] = *reinterpret_cast<const uint16_t*>(p + j * kKv4BlockBytes + kKv4VScale + lane * 2);
+        }
+    };
+
+    // A warp takes every eighth step of the CTA's range.  The next step's K
+    // is on its way from the moment the current K is used up, its V likewise,
+    // and the page number after that one step longer: 9 KB a warp in flight
+    // at no registers beyond one step's.
+    bool any_bad = false;
+    int u = u0 + warp, page = lookup(u), next = lookup(u + kWarps);
+    if (u < u1) {
+        load_k(at(u, page));
+        load_v(at(u, page));
+    }
+    for (; u < u1; u += kWarps) {
+        const bool more = u + kWarps < u1, bad = page < 0;
+        const int key0 = key_of(u);
+        page = next;
+        const uint8_t* np = at(more ? u + kWarps : u, page);
+        next = lookup(u + 2 * kWarps);
+        any_bad |= bad;
         // S^T
-        float c[NB][4];
+        float c[NB][2][4];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
-        const uint32_t k0[4] = {z.k0.x, z.k0.y, z.k0.z, z.k0.w}, k1[4] = {z.k1.x, z.k1.y, z.k1.z, z.k1.w};
+        for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            // words 0, 1 are the quarter's first 16-dim group, 2, 3 the second
-            const Scale2 s0 = scale2(__byte_perm(z.ks, 0, w < 2 ? 0x4040 : 0x4141));
-            const Scale2 s1 = scale2(__byte_perm(z.ks, 0, w < 2 ? 0x4242 : 0x4343));
-            const uint32_t a0 = field<0>(k0[w], s0), a1 = field<0>(k1[w], s1);
-            const uint32_t a2 = field<1>(k0[w], s0), a3 = field<1>(k1[w], s1);
-            const uint32_t a4 = field<2>(k0[w], s0), a5 = field<2>(k1[w], s1);
-            const uint32_t a6 = field<3>(k0[w], s0), a7 = field<3>(k1[w], s1);
+            for (int e = 0; e < 2; ++e) c[i][e][0] = c[i][e][1] = c[i][e][2] = c[i][e][3] = 0.f;
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                mma16816(c[i], a0, a1, a2, a3, qf[i][4 * w], qf[i][4 * w + 1]);
-                mma16816(c[i], a4, a5, a6, a7, qf[i][4 * w + 2], qf[i][4 * w + 3]);
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t k0[4] = {kc[2 * e].x, kc[2 * e].y, kc[2 * e].z, kc[2 * e].w};
+            const uint32_t k1[4] = {kc[2 * e + 1].x, kc[2 * e + 1].y, kc[2 * e + 1].z, kc[2 * e + 1].w};
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {          // the quarter's two 16-dim groups
+                const Scale2 s0 = scale2(__byte_perm(ks[2 * e], 0, d ? 0x4141 : 0x4040));
+                const Scale2 s1 = scale2(__byte_perm(ks[2 * e + 1], 0, d ? 0x4141 : 0x4040));
+#pragma unroll
+                for (int w = 2 * d; w < 2 * d + 2; ++w) {
+                    const uint32_t a0 = field<0>(k0[w], s0), a1 = field<0>(k1[w], s1);
+                    const uint32_t a2 = field<1>(k0[w], s0), a3 = field<1>(k1[w], s1);
+                    const uint32_t a4 = field<2>(k0[w], s0), a5 = field<2>(k1[w], s1);
+                    const uint32_t a6 = field<3>(k0[w], s0), a7 = field<3>(k1[w], s1);
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) {
+                        mma16816(c[i][e], a0, a1, a2, a3, qf[i][4 * w], qf[i][4 * w + 1]);
+                        mma16816(c[i][e], a4, a5, a6, a7, qf[i][4 * w + 2], qf[i][4 * w + 3]);
+                    }
+                }
             }
         }
-        // masks, running max, P
-        const bool whole = !z.bad && z.key + kKeys <= first.hi &&
-                           (z.key >= last.lo || z.key + kKeys <= P.sink_rows);
+        if (more) load_k(np);
+        // masks
+        if (bad || key0 + kKeys > first.hi || (key0 < last.lo && key0 + kKeys > P.sink_rows)) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const int r = min(r0 + 8 * i + 2 * t + a, rows - 1);
+                    const Sees y = sees(P, start + r / P.group, end);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + g + 8 * e;
+                        if (bad || key >= y.hi || (key < y.lo && key >= P.sink_rows))
+                            c[i][e >> 1][a + 2 * (e & 1)] = -INFINITY;
+                    }
+                }
+        }
+        // The max moves only when some score passes it by more than 2^8 (or a
+        // row sees its first key): P then stays below 2^8, far inside fp32 and
+        // bf16, and most steps need no reduction over the keys.
         bool rise = false;
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int key = z.key + g + 8 * (e >> 1);
-                c[i][e] *= P.scale_log2;
-                if (!whole && (z.bad || key >= hi[i][e & 1] || (key < lo[i][e & 1] && key >= P.sink_rows)))
-                    c[i][e] = -INFINITY;
-                rise |= c[i][e] > m[i][e & 1] + kRise;
+            for (int a = 0; a < 2; ++a) {
+                const float top = fmaxf(fmaxf(c[i][0][a], c[i][0][a + 2]), fmaxf(c[i][1][a], c[i][1][a + 2]));
+                rise |= top > m[i][a] + P.rise;
             }
-        // The max moves only when some score passes it by more than 2^8 (or a
-        // row sees its first key): P then stays below 2^8, far inside fp32 and
-        // bf16, and most steps need no reduction over the keys.
         if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
-                    float top = fmaxf(c[i][a], c[i][a + 2]);
+                    float top = fmaxf(fmaxf(c[i][0][a], c[i][0][a + 2]), fmaxf(c[i][1][a], c[i][1][a + 2]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                     const float up = fmaxf(m[i][a], top);
-                    const float f = up == m[i][a] ? 1.f : ex2(m[i][a] - up);
+                    const float f = up == m[i][a] ? 1.f : ex2((m[i][a] - up) * P.scale_log2);
                     m[i][a] = up;
                     l[i][a] *= f;
 #pragma unroll
@@ -212,57 +236,49 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
                     }
                 }
         }
-        uint32_t p0[NB], p1[NB];
+        uint32_t p[NB][4];
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const float ma = m[i][0] == -INFINITY ? 0.f : m[i][0], mb = m[i][1] == -INFINITY ? 0.f : m[i][1];
-            const float e0 = ex2(c[i][0] - ma), e1 = ex2(c[i][1] - mb);
-            const float e2 = ex2(c[i][2] - ma), e3 = ex2(c[i][3] - mb);
-            l[i][0] += e0 + e2;
-            l[i][1] += e1 + e3;
-            // P to bf16 (a tensor-core operand): half a step, 2^-9 of each
-            // weight, without bias; the sum l keeps 32 bits
-            p0[i] = transpose8(pack2(e0, e1));
-            p1[i] = transpose8(pack2(e2, e3));
+            const float na0 = m[i][0] == -INFINITY ? 0.f : -m[i][0] * P.scale_log2;
+            const float na1 = m[i][1] == -INFINITY ? 0.f : -m[i][1] * P.scale_log2;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p0 = ex2(fmaf(c[i][e >> 1][2 * (e & 1)], P.scale_log2, na0));
+                const float p1 = ex2(fmaf(c[i][e >> 1][2 * (e & 1) + 1], P.scale_log2, na1));
+                l[i][0] += p0;
+                l[i][1] += p1;
+                // P to bf16 (a tensor-core operand): at most 2^-8 of each
+                // weight, without bias; the sum l keeps 32 bits
+                p[i][e] = transpose8(pack2(p0, p1));
+            }
         }
         // O^T: word d of a row holds dims 16g + 8d + 2i (low half's field i)
         // and + 1 (high half's); pairing two rows' halves puts two keys of one
         // dim into a register
-        const Scale2 s0 = scale2(__byte_perm(z.vs, 0, 0x4140)), s1 = scale2(__byte_perm(z.vs, 0, 0x4342));
-        const uint32_t va[2] = {z.v0.x, z.v0.y}, vb[2] = {z.v0.z, z.v0.w};
-        const uint32_t vc[2] = {z.v1.x, z.v1.y}, vd[2] = {z.v1.z, z.v1.w};
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
-            const uint32_t e0 = __byte_perm(va[d], vb[d], 0x5410), o0 = __byte_perm(va[d], vb[d], 0x7632);
-            const uint32_t e1 = __byte_perm(vc[d], vd[d], 0x5410), o1 = __byte_perm(vc[d], vd[d], 0x7632);
-            auto step = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+        for (int e = 0; e < 2; ++e) {
+            const uint4 v0 = vc[2 * e], v1 = vc[2 * e + 1];
+            const Scale2 s0 = scale2(__byte_perm(vs[2 * e], 0, 0x4140));
+            const Scale2 s1 = scale2(__byte_perm(vs[2 * e + 1], 0, 0x4140));
 #pragma unroll
-                for (int i = 0; i < NB; ++i) mma16816(o[i][j], a0, a1, a2, a3, p0[i], p1[i]);
-            };
-            step(4 * d, field<0>(e0, s0), field<0>(o0, s0), field<0>(e1, s1), field<0>(o1, s1));
-            step(4 * d + 1, field<1>(e0, s0), field<1>(o0, s0), field<1>(e1, s1), field<1>(o1, s1));
-            step(4 * d + 2, field<2>(e0, s0), field<2>(o0, s0), field<2>(e1, s1), field<2>(o1, s1));
-            step(4 * d + 3, field<3>(e0, s0), field<3>(o0, s0), field<3>(e1, s1), field<3>(o1, s1));
+            for (int d = 0; d < 2; ++d) {
+                const uint32_t e0 = __byte_perm(d ? v0.y : v0.x, d ? v0.w : v0.z, 0x5410);
+                const uint32_t o0 = __byte_perm(d ? v0.y : v0.x, d ? v0.w : v0.z, 0x7632);
+                const uint32_t e1 = __byte_perm(d ? v1.y : v1.x, d ? v1.w : v1.z, 0x5410);
+                const uint32_t o1 = __byte_perm(d ? v1.y : v1.x, d ? v1.w : v1.z, 0x7632);
+                auto step = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) mma16816(o[i][j], a0, a1, a2, a3, p[i][2 * e], p[i][2 * e + 1]);
+                };
+                step(4 * d, field<0>(e0, s0), field<0>(o0, s0), field<0>(e1, s1), field<0>(o1, s1));
+                step(4 * d + 1, field<1>(e0, s0), field<1>(o0, s0), field<1>(e1, s1), field<1>(o1, s1));
+                step(4 * d + 2, field<2>(e0, s0), field<2>(o0, s0), field<2>(e1, s1), field<2>(o1, s1));
+                step(4 * d + 3, field<3>(e0, s0), field<3>(o0, s0), field<3>(e1, s1), field<3>(o1, s1));
+            }
         }
-    };
-
-    // A warp takes every eighth step of the CTA's range; the next step's bytes
-    // and the page number after that are in flight while one is computed.
-    bool bad = false;
-    int u = u0 + warp;
-    if (u < u1) {
-        Step cur = load(u, lookup(u));
-        int page = lookup(u + kWarps);
-        for (; u < u1; u += kWarps) {
-            Step nxt = cur;
-            if (u + kWarps < u1) nxt = load(u + kWarps, page);
-            page = lookup(u + 2 * kWarps);
-            bad |= cur.bad;
-            compute(cur);
-            cur = nxt;
-        }
+        if (more) load_v(np);
     }
-    if (bad && lane == 0) atomicOr(P.status, KVP_STATUS_MAP);
+    if (any_bad && lane == 0) atomicOr(P.status, KVP_STATUS_MAP);
 
     // Join the warps: l over the lanes of a column, then (O, m, l) over the warps.
 #pragma unroll
@@ -274,7 +290,7 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
             l[i][a] += __shfl_xor_sync(0xffffffffu, l[i][a], 16);
             const int q = 8 * i + 2 * t + a;
             if (g == 0) {
-                sm.m[warp][q] = m[i][a];
+                sm.m[warp][q] = m[i][a] * P.scale_log2;
                 sm.l[warp][q] = l[i][a];
             }
 #pragma unroll
@@ -305,11 +321,14 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
 }
 
 // ------------------------------------------------------------- joining splits
-// One warp per (sequence, K/V head, row), four dims a lane.
+// One warp per (sequence, K/V head, row), four dims a lane.  Launched while
+// the splits still run (programmatic stream serialization), so that its own
+// launch costs no time after them.
 __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
     const Kv4Span& s = P.span;
     const int lane = threadIdx.x & 31;
     const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    cudaGridDependencySynchronize();                  // the partials are complete and visible
     if (w >= (long long)s.batch * s.kv_heads * P.max_rows) return;
     const int r = (int)(w % P.max_rows);
     const int h = (int)(w / P.max_rows % s.kv_heads), b = (int)(w / P.max_rows / s.kv_heads);
@@ -369,6 +388,7 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     P.window_rows = a.window ? std::min<long long>((long long)a.window * a.tokens, 1LL << 31) : 0;
     P.sink_rows = (int)std::min<long long>((long long)a.sinks * a.tokens, cap);
     P.scale_log2 = 1.4426950408889634f / sqrtf((float)kKv4Head);
+    P.rise = kRise / P.scale_log2;
 
     const int nb = P.max_rows > 8 ? 2 : 1;
     P.row_tiles = (P.max_rows + 8 * nb - 1) / (8 * nb);
@@ -376,11 +396,13 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     // Key steps of a row tile, at most (starts on the device: the capacity's).
     long long keys = s.starts ? cap : (long long)s.start + s.rows;
     if (a.window) {
-        const long long span = (long long)(8 * nb / P.group + 2 + a.tokens) + (long long)P.window_rows + P.sink_rows + 32;
+            const long long span = (long long)(8 * nb / P.group + 2 + a.tokens) + (long long)P.window_rows + P.sink_rows + 32;
         keys = std::min(keys, span);
     }
-    // Two CTAs an SM; a split keeps a step for each warp.
-    const long long want = (2LL * sm_count() + units - 1) / units;
+    // As many splits as fill two CTAs an SM (one more CTA would wait for a
+    // second round: 37 us against 25 at 32768 keys x 12 heads), a step for
+    // each warp of a split at least.
+    const long long want = 2LL * sm_count() / units;
     const long long most = (keys + kKeys * kWarps - 1) / (kKeys * kWarps);
     P.splits = (int)std::max<long long>(1, std::min(std::min(want, most), 256LL));
     const long long grid = units * P.splits;
@@ -401,8 +423,16 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     if (ws) {
         if (launched == KVP_OK) {
             const long long warps = slots / P.splits;
-            attn_kv4_join_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(P);
-            const cudaError_t e = cudaGetLastError();
+            cudaLaunchAttribute early;
+            early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            early.val.programmaticStreamSerializationAllowed = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)((warps + 7) / 8));
+            cfg.blockDim = dim3(256);
+            cfg.stream = stream;
+            cfg.attrs = &early;
+            cfg.numAttrs = 1;
+            const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel, P);
             if (e != cudaSuccess) launched = cuda_status(e, "attn_kv4 join");
         }
         const cudaError_t e = cudaFreeAsync(ws, stream);

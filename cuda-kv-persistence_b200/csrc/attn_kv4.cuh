@@ -18,7 +18,8 @@ struct Kv4Params {
     int sink_rows;           // sinks * tokens, at most the capacity
     int group, max_rows;     // query heads per K/V head; rows * group
     int tokens, row_tiles, splits;
-    float scale_log2;
+    float scale_log2;        // log2(e) / sqrt(128)
+    float rise;              // kRise in score units
 };
 
 namespace kv4_dev {

@@ -127,7 +127,9 @@ __device__ __forceinline__ Scale2 scale2(uint32_t b2) {
 // (1 + c/128) * 128 s - 136 s = (c - 8) s, exact.
 template <int i>
 __device__ __forceinline__ uint32_t field(uint32_t w, const Scale2& s) {
-    return bf2_fma(((w >> (4 * i)) & 0x000F000Fu) | 0x3F803F80u, s.hi, s.lo);
+    uint32_t x;   // one lop3: (w & mask) | one
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> (4 * i)), "r"(0x000F000Fu), "r"(0x3F803F80u));
+    return bf2_fma(x, s.hi, s.lo);
 }
 
 }  // namespace kv4_dev

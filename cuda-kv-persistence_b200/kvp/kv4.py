@@ -20,17 +20,22 @@ Everything is queued on the current stream of the tensors' device, or on
 
 from __future__ import annotations
 
-import ctypes as C
+from ctypes import byref
+
+import torch
 
 from ._lib import Kv4Attn, Kv4Rows, Kv4Span, KvpError, check, lib
 
 PAGE_ROWS = 128
 PAGE_HEAD_BYTES = 18432
 
+_ROW_TYPES = (torch.bfloat16, torch.float32)
+_Q_TYPES = (torch.bfloat16,)
+_MAX_INT = 2 ** 31
+
 
 def alloc_pages(n_pages: int, kv_heads: int, device="cuda"):
     """An unwritten pool (any bytes stand for finite values)."""
-    import torch
     return torch.empty(n_pages, kv_heads, PAGE_HEAD_BYTES, dtype=torch.uint8, device=device)
 
 
@@ -42,78 +47,89 @@ def _rows3(t, name: str, dtypes, heads: int):
     """(batch, rows, row stride, batch stride) of a row tensor."""
     if t.dtype not in dtypes:
         _bad(f"{name} is {t.dtype}, expected one of {[str(d) for d in dtypes]}")
-    if t.dim() == 2:
-        b, (n, d), rs, bs = 1, t.shape, t.stride(0), 0
-    elif t.dim() == 3:
-        (b, n, d), rs, bs = t.shape, t.stride(1), t.stride(0)
+    shape, strides = t.shape, t.stride()
+    if len(shape) == 3:
+        b, n, d = shape
+        bs, rs, es = strides
+    elif len(shape) == 2:
+        n, d = shape
+        rs, es = strides
+        b, bs = 1, 0
     else:
         _bad(f"{name} must be [rows, heads * 128] or [batch, rows, heads * 128]")
-    if d != heads * 128 or t.stride(-1) != 1:
-        _bad(f"{name} needs {heads} heads of 128 contiguous elements, got {tuple(t.shape)}")
+    if d != heads * 128 or es != 1:
+        _bad(f"{name} needs {heads} heads of 128 contiguous elements, got {tuple(shape)}")
     # the strides of single rows and sequences mean nothing
     return b, n, rs if n > 1 else d, bs if b > 1 else 0
 
 
-def _span(pages, batch: int, rows: int, page_map, start: int, starts, counts, tensors):
-    import torch
-    if pages.dtype != torch.uint8 or pages.dim() != 3 or pages.shape[2] != PAGE_HEAD_BYTES or \
+def _pool(pages):
+    """(n_pages, kv_heads) of a pool."""
+    shape = pages.shape
+    if pages.dtype != torch.uint8 or len(shape) != 3 or shape[2] != PAGE_HEAD_BYTES or \
             not pages.is_contiguous():
         _bad(f"pages must be a contiguous uint8 [n_pages, kv_heads, {PAGE_HEAD_BYTES}] tensor")
-    dev = pages.device
-    if dev.type != "cuda":
+    return shape[0], shape[1]
+
+
+def _batch_ints(t, name: str, batch: int, dev: int) -> int:
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != batch or not t.is_contiguous():
+        _bad(f"{name} must be a contiguous int32 [{batch}] tensor")
+    if t.get_device() != dev:
+        _bad(f"tensors on {t.device} and cuda:{dev}")
+    return t.data_ptr()
+
+
+def _span(pages, batch: int, rows: int, page_map, start: int, starts, counts, a, b):
+    n_pages, kv_heads = pages.shape[0], pages.shape[1]
+    dev = pages.get_device()
+    if dev < 0:
         _bad("pages must be a CUDA tensor")
-    n_pages = pages.shape[0]
+    for t in (a, b):
+        if t is not None and t.get_device() != dev:
+            _bad(f"tensors on {t.device} and cuda:{dev}")
     if page_map is None:
-        stride = n_pages // batch if batch else n_pages
+        stride, map_ptr = n_pages // max(batch, 1), 0
     else:
         if page_map.dtype != torch.int32 or page_map.dim() != 2 or page_map.shape[0] != batch or \
                 not page_map.is_contiguous():
             _bad(f"page_map must be a contiguous int32 [{batch}, pages] tensor")
-        stride = page_map.shape[1]
-    for t, name in ((starts, "starts"), (counts, "counts")):
-        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (batch,) or
-                              not t.is_contiguous()):
-            _bad(f"{name} must be a contiguous int32 [{batch}] tensor")
-    for t in (page_map, starts, counts, *tensors):
-        if t is not None and t.device != dev:
-            _bad(f"tensors on {t.device} and {dev}")
-    if not (0 <= start < 2 ** 31 and rows < 2 ** 31):
-        _bad(f"start {start}, rows {rows} out of range")
-    return Kv4Span(pages.data_ptr(), 0 if page_map is None else page_map.data_ptr(),
-                   0 if starts is None else starts.data_ptr(),
-                   0 if counts is None else counts.data_ptr(), n_pages, pages.shape[1], batch,
-                   stride, start, rows)
+        if page_map.get_device() != dev:
+            _bad(f"tensors on {page_map.device} and cuda:{dev}")
+        stride, map_ptr = page_map.shape[1], page_map.data_ptr()
+    if not (0 <= start < _MAX_INT and rows < _MAX_INT and stride < _MAX_INT):
+        _bad(f"start {start}, rows {rows} or {stride} pages out of range")
+    return Kv4Span(pages.data_ptr(), map_ptr, _batch_ints(starts, "starts", batch, dev),
+                   _batch_ints(counts, "counts", batch, dev), n_pages, kv_heads, batch, stride, start, rows)
 
 
-def _call(fn, what, dev, stream, *args):
-    import torch
+def _call(fn, what, pages, stream, *args):
+    dev = pages.get_device()
     if stream is None:
         stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, int(stream)), what)
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, int(stream)), what)
+            rc = fn(*args, stream)
+    if rc < 0:
+        check(rc, what)
 
 
 def _kv(pages, k, v, page_map, start, starts, counts):
-    import torch
     some = k if k is not None else v
     if some is None:
         _bad("no rows")
-    if pages.dim() != 3:
-        _bad("pages must be [n_pages, kv_heads, bytes]")
-    heads = pages.shape[1]
-    types = (torch.bfloat16, torch.float32)
-    shape = _rows3(some, "k" if k is not None else "v", types, heads)
-    if k is not None and v is not None and (_rows3(v, "v", types, heads) != shape or
+    heads = _pool(pages)[1]
+    b, n, rs, bs = shape = _rows3(some, "k" if k is not None else "v", _ROW_TYPES, heads)
+    if k is not None and v is not None and (_rows3(v, "v", _ROW_TYPES, heads) != shape or
                                             k.dtype != v.dtype):
         _bad("k and v must agree in shape, strides and type")
-    b, n, rs, bs = shape
-    span = _span(pages, b, n, page_map, start, starts, counts, (k, v))
-    rows = Kv4Rows(0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), rs, bs,
-                   some.element_size())
-    return span, rows
+    span = _span(pages, b, n, page_map, start, starts, counts, k, v)
+    return span, Kv4Rows(0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), rs, bs,
+                         some.element_size())
 
 
 def write(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=None,
@@ -122,14 +138,14 @@ def write(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=Non
     if k is None or v is None:
         _bad("write needs k and v")
     span, rows = _kv(pages, k, v, page_map, start, starts, counts)
-    _call(lib().kvp_kv4_write, "kvp_kv4_write", pages.device, stream, C.byref(span), C.byref(rows))
+    _call(lib().kvp_kv4_write, "kvp_kv4_write", pages, stream, byref(span), byref(rows))
 
 
 def read(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=None,
          stream=None) -> None:
     """Fills k and v (bf16 or fp32; either may be None) with the rows' values."""
     span, rows = _kv(pages, k, v, page_map, start, starts, counts)
-    _call(lib().kvp_kv4_read, "kvp_kv4_read", pages.device, stream, C.byref(span), C.byref(rows))
+    _call(lib().kvp_kv4_read, "kvp_kv4_read", pages, stream, byref(span), byref(rows))
 
 
 def attn(q, pages, out, *, heads: int, page_map=None, start: int = 0, starts=None, counts=None,
@@ -138,12 +154,11 @@ def attn(q, pages, out, *, heads: int, page_map=None, start: int = 0, starts=Non
     position p, in frame f = p // tokens, sees the cached rows up to the end of
     its frame (and of this call's rows) that lie in the last `window` frames (0: all) or the
     first `sinks` frames.  The call's own rows are keys: write them first."""
-    import torch
-    bf = (torch.bfloat16,)
-    b, n, qr, qb = _rows3(q, "q", bf, heads)
-    ob, on, orow, obatch = _rows3(out, "out", bf, heads)
-    if (ob, on) != (b, n):
+    _pool(pages)
+    b, n, qr, qb = _rows3(q, "q", _Q_TYPES, heads)
+    ob, on, orow, obatch = _rows3(out, "out", _Q_TYPES, heads)
+    if ob != b or on != n:
         _bad("q and out must agree in shape")
-    span = _span(pages, b, n, page_map, start, starts, counts, (q, out))
+    span = _span(pages, b, n, page_map, start, starts, counts, q, out)
     a = Kv4Attn(q.data_ptr(), out.data_ptr(), qr, qb, orow, obatch, heads, tokens, window, sinks)
-    _call(lib().kvp_attn_kv4, "kvp_attn_kv4", pages.device, stream, C.byref(span), C.byref(a))
+    _call(lib().kvp_attn_kv4, "kvp_attn_kv4", pages, stream, byref(span), byref(a))
