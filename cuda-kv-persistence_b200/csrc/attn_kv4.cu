@@ -370,6 +370,22 @@ int sm_count() {
     return n > 0 ? n : 148;
 }
 
+// Splits of the pages of a 256-row tile: minimise rounds of one CTA an SM x
+// (pages of a split + a fixed cost of about 4 pages: prologue, epilogue, join).
+int tile_splits(long long units, int pages, int sms) {
+    int best = 1;
+    long long best_cost = -1;
+    for (int c = 1; c <= 64 && c <= (pages + 1) / 2; ++c) {
+        const long long rounds = (units * c + sms - 1) / sms;
+        const long long cost = rounds * ((pages + c - 1) / c + (c > 1 ? 4 : 2));
+        if (best_cost < 0 || cost < best_cost) {
+            best_cost = cost;
+            best = c;
+        }
+    }
+    return best;
+}
+
 }  // namespace
 
 int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStream_t stream) {
@@ -390,21 +406,28 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     P.scale_log2 = 1.4426950408889634f / sqrtf((float)kKv4Head);
     P.rise = kRise / P.scale_log2;
 
-    const int nb = P.max_rows > 8 ? 2 : 1;
-    P.row_tiles = (P.max_rows + 8 * nb - 1) / (8 * nb);
+    // Up to 16 rows of a K/V head fit the N side of the mma.sync kernel.
+    const bool tiles = P.max_rows > 16;
+    const int nb = P.max_rows > 8 ? 2 : 1, tile_rows = tiles ? 256 : 8 * nb;
+    P.row_tiles = (P.max_rows + tile_rows - 1) / tile_rows;
     const long long units = (long long)s.batch * s.kv_heads * P.row_tiles;
-    // Key steps of a row tile, at most (starts on the device: the capacity's).
+    // Keys of a row tile, at most (starts on the device: the capacity's).
     long long keys = s.starts ? cap : (long long)s.start + s.rows;
     if (a.window) {
-            const long long span = (long long)(8 * nb / P.group + 2 + a.tokens) + (long long)P.window_rows + P.sink_rows + 32;
+        const long long span = (long long)(tile_rows / P.group + 2 + (long long)a.tokens) + P.window_rows + P.sink_rows;
         keys = std::min(keys, span);
     }
-    // As many splits as fill two CTAs an SM (one more CTA would wait for a
-    // second round: 37 us against 25 at 32768 keys x 12 heads), a step for
-    // each warp of a split at least.
-    const long long want = 2LL * sm_count() / units;
-    const long long most = (keys + kKeys * kWarps - 1) / (kKeys * kWarps);
-    P.splits = (int)std::max<long long>(1, std::min(std::min(want, most), 256LL));
+    const int sms = sm_count();
+    if (tiles) {
+        P.splits = tile_splits(units, (int)((keys + kKv4PageRows - 1) / kKv4PageRows), sms);
+    } else {
+        // As many splits as fill two CTAs an SM (one more CTA would wait for a
+        // second round: 37 us against 25 at 32768 keys x 12 heads), a step for
+        // each warp of a split at least.
+        const long long want = 2LL * sms / units;
+        const long long most = (keys + kKeys * kWarps - 1) / (kKeys * kWarps);
+        P.splits = (int)std::max<long long>(1, std::min(std::min(want, most), 256LL));
+    }
     const long long grid = units * P.splits;
     if (grid > 0x7fffffffLL) {
         set_error("attn_kv4: too many rows for one launch");
@@ -419,7 +442,9 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
         P.ws_o = static_cast<float*>(ws);
         P.ws_ml = P.ws_o + slots * kKv4Head;
     }
-    int launched = nb == 1 ? launch_rows<1>(P, (unsigned)grid, stream) : launch_rows<2>(P, (unsigned)grid, stream);
+    int launched = tiles   ? launch_kv4_tiles(P, (unsigned)grid, stream)
+                   : nb == 1 ? launch_rows<1>(P, (unsigned)grid, stream)
+                             : launch_rows<2>(P, (unsigned)grid, stream);
     if (ws) {
         if (launched == KVP_OK) {
             const long long warps = slots / P.splits;

@@ -1,0 +1,480 @@
+// Attention over the 4-bit K/V cache for many query rows: tcgen05 tensor
+// cores, the cache expanded to bf16 on its way into shared memory.
+//
+// Bound by the two products: 4 * 128 flops a (query row, key), against 144
+// bytes a key that every 256 query rows read again from L2.  CTA = two
+// 128-row query tiles of one K/V head (rows r = i * group + g, so grouped
+// heads fill a tile) x a range of 128-key pages.  Warp roles (384 threads):
+//   warps 0, 2, 3   expand the cache: units of 32 rows of K or V in turn,
+//                   16-byte words from global memory (one unit ahead), fields
+//                   to bf16 in registers, 16-byte stores into the 128B-
+//                   swizzled tiles that TMA would write from bf16 rows (K
+//                   K-major, V MN-major); the words of half the lanes change
+//                   places so that no store conflicts
+//   warp 1          TMEM and the single-thread MMA issuer: S0_j, PV1_{j-1},
+//                   S1_j, PV0_j
+//   warps 4-7, 8-11 softmax of query tile 0 and 1, a row a thread, P kept in
+//                   TMEM, the running max raised only when a row's sum
+//                   overgrows
+// TMEM: S0 | S1 | O0 | O1, 128 columns each; P overlays S's first 64.
+// Every wait is bounded (sm100_ptx.h).
+#include <cstring>
+
+#include "attn_kv4.cuh"
+#include "attn_mma_sm100.cuh"
+#include "attn_softmax_sm100.cuh"
+#include "kv4.h"
+
+namespace kvp {
+
+namespace {
+
+using namespace ptx;
+using namespace attn_dev;
+using namespace kv4_dev;
+
+constexpr int kThreads = 384;
+constexpr int kBN = kKv4PageRows;             // keys of a tile
+constexpr int kKStages = 2, kVStages = 3;
+constexpr uint32_t kPanel = 128 * 128;        // one [128 rows][64 bf16] swizzled panel
+constexpr uint32_t kTileBytes = 2 * kPanel;
+constexpr int kRegsLow = 104, kRegsHigh = 200;   // warps 0-3, 4-11
+static_assert(kRegsLow * 128 + 2 * kRegsHigh * 128 <= 65536, "register split exceeds the SM");
+constexpr float kRedoSum = 256.f;             // a tile row sum above this takes the new max
+constexpr int kUnits = 8;                     // of a tile: K rows 0-31, 32-63, .., then V's
+constexpr int kExpanders = 3;
+
+struct __align__(1024) Smem {
+    uint8_t q[2][kTileBytes];
+    uint8_t k[kKStages][kTileBytes];
+    uint8_t v[kVStages][kTileBytes];
+    uint64_t bar_q[2];
+    uint64_t bar_kfull[kKStages], bar_kempty[kKStages];
+    uint64_t bar_vfull[kVStages], bar_vempty[kVStages];
+    uint64_t bar_s_full[2];     // S_q(j) landed (and, by issue order, PV_q(j-1) too)
+    uint64_t bar_p_full[2];     // P_q(j) in TMEM, S_q(j) read, O_q rescaled
+    uint64_t bar_o_done[2];     // last PV_q landed
+    uint64_t bar_mma_done;      // every issued MMA landed (TMEM may be freed)
+    uint32_t tmem_base;
+    int abort_flag;
+    // the CTA's item, for what the softmax seldom needs (not held in registers)
+    volatile int batch, head, rows, row0, split, u0, na, b0, any_bad, releaser;
+};
+
+// The four words and scale bytes of a lane's 16 bytes as four bf16 chunks.
+__device__ __forceinline__ void expand4(uint8_t* tile, const uint32_t (&off)[4], uint32_t w0, uint32_t w1,
+                                        uint32_t w2, uint32_t w3, const Scale2& s01, const Scale2& s23) {
+    *reinterpret_cast<uint4*>(tile + off[0]) = make_uint4(field<0>(w0, s01), field<1>(w0, s01), field<2>(w0, s01), field<3>(w0, s01));
+    *reinterpret_cast<uint4*>(tile + off[1]) = make_uint4(field<0>(w1, s01), field<1>(w1, s01), field<2>(w1, s01), field<3>(w1, s01));
+    *reinterpret_cast<uint4*>(tile + off[2]) = make_uint4(field<0>(w2, s23), field<1>(w2, s23), field<2>(w2, s23), field<3>(w2, s23));
+    *reinterpret_cast<uint4*>(tile + off[3]) = make_uint4(field<0>(w3, s23), field<1>(w3, s23), field<2>(w3, s23), field<3>(w3, s23));
+}
+
+__global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __grid_constant__ Kv4Params P) {
+    extern __shared__ uint8_t smem_raw[];
+    cudaTriggerProgrammaticLaunchCompletion();    // the join may be launched; it waits for the data
+    if (reinterpret_cast<uintptr_t>(smem_raw) & 1023) {
+        if (threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_ALIGN);
+        return;
+    }
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    const Kv4Span& s = P.span;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // CTA = (split, query tile pair, K/V head, sequence), split fastest, last rows
+    // (the longest spans) first
+    long long x = blockIdx.x;
+    const int split = (int)(x % P.splits);
+    x /= P.splits;
+    const int h = (int)(x % s.kv_heads);
+    x /= s.kv_heads;
+    const int b = (int)(x % s.batch);
+    const int r0 = (P.row_tiles - 1 - (int)(x / s.batch)) * 256;
+    int start, count;
+    if (!sequence(s, b, start, count)) {
+        if (threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_MAP);
+        return;
+    }
+    const int rows = count * P.group;
+    if (r0 >= rows) return;
+    const int end = start + count;
+    const Sees first = sees(P, start + r0 / P.group, end);
+    const Sees last = sees(P, start + (min(r0 + 256, rows) - 1) / P.group, end);
+    // pages: those of the sinks below the window, then the window's
+    const int b0 = first.lo / kBN, na = min((min(P.sink_rows, last.hi) + kBN - 1) / kBN, b0);
+    const int total = na + (last.hi + kBN - 1) / kBN - b0, per = (total + P.splits - 1) / P.splits;
+    const int u0 = min(split * per, total), n_tiles = min(u0 + per, total) - u0;
+    const bool two = r0 + 128 < rows;             // the second query tile has rows
+    auto page_pos = [&](int j) {                  // position page of the CTA's tile j
+        const int u = u0 + j;
+        return u < na ? u : u - na + b0;
+    };
+    auto lookup = [&](int j) { return j < n_tiles ? page_of(s, b, page_pos(j)) : 0; };
+
+    if (threadIdx.x == 0) {
+        for (int q = 0; q < 2; ++q) {
+            mbar_init(&sm.bar_q[q], 128);
+            mbar_init(&sm.bar_s_full[q], 1);
+            mbar_init(&sm.bar_p_full[q], 128);
+            mbar_init(&sm.bar_o_done[q], 1);
+        }
+        for (int i = 0; i < kKStages; ++i) {
+            mbar_init(&sm.bar_kfull[i], kUnits / 2);
+            mbar_init(&sm.bar_kempty[i], 1);
+        }
+        for (int i = 0; i < kVStages; ++i) {
+            mbar_init(&sm.bar_vfull[i], kUnits / 2);
+            mbar_init(&sm.bar_vempty[i], 1);
+        }
+        mbar_init(&sm.bar_mma_done, 1);
+        sm.abort_flag = 0;
+        sm.batch = b;
+        sm.head = h;
+        sm.rows = rows;
+        sm.row0 = r0;
+        sm.split = split;
+        sm.u0 = u0;
+        sm.na = na;
+        sm.b0 = b0;
+        sm.any_bad = 0;
+        sm.releaser = two ? 256 : 128;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async_smem();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&sm.tmem_base)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    bool bad = false;
+    for (int j = threadIdx.x; j < n_tiles; j += kThreads) bad |= lookup(j) < 0;
+    tc_fence_before();
+    const bool any_bad = __syncthreads_or(bad);   // some page is not in the pool: its keys are masked
+    tc_fence_after();
+    if (any_bad) sm.any_bad = 1;                  // (every thread writes the same, its own reads follow)
+    const uint32_t tmem = sm.tmem_base;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+        if (warp != 1) {
+            // ============================ expanders ===========================
+            const int g = lane >> 2, t = lane & 3;
+            // K: row g of a block, quarter t, words in the order i ^ (t & 2).
+            // V: rows 2t and 2t + 1, group g, words of a row in the order e ^ (g & 1).
+            uint32_t koff[4], voff[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                koff[i] = (t >> 1) * kPanel + g * 128 + ((((t & 1) * 4) ^ (t & 2) ^ g ^ i) << 4);
+                voff[i] = (g >> 2) * kPanel + (2 * t + (i >> 1)) * 128 +
+                          ((((g & 3) * 2) ^ (g & 1) ^ (2 * t) ^ (i >> 1) ^ (i & 1)) << 4);
+            }
+            const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
+            const uint8_t* head = static_cast<const uint8_t*>(s.pages) + h * kKv4PageHeadBytes;
+            const int units = n_tiles * kUnits;
+            uint4 c[4];
+            uint32_t sc[4];
+            auto load = [&](int n, int page) {
+                const int part = (n >> 2) & 1;
+                const uint8_t* p = head + (unsigned long long)(uint32_t)max(page, 0) * page_bytes +
+                                   (n & 3) * 4 * kKv4BlockBytes;
+                const uint8_t* pc = p + (part ? kKv4VCode : 0) + lane * 16;
+                const uint8_t* ps = p + (part ? kKv4VScale : kKv4KScale) + lane * 2;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    c[i] = *reinterpret_cast<const uint4*>(pc + i * kKv4BlockBytes);
+                    sc[i] = *reinterpret_cast<const uint16_t*>(ps + i * kKv4BlockBytes);
+                }
+            };
+            int n = warp == 0 ? 0 : warp - 1;
+            int page = lookup(n / kUnits), page1 = lookup((n + kExpanders) / kUnits);
+            if (n < units) load(n, page);
+            for (; n < units; n += kExpanders) {
+                page = page1;
+                page1 = lookup((n + 2 * kExpanders) / kUnits);
+                uint4 cc[4];
+                uint32_t ss[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    cc[i] = c[i];
+                    ss[i] = sc[i];
+                }
+                if (n + kExpanders < units) load(n + kExpanders, page);
+                const int j = n / kUnits, part = (n >> 2) & 1;
+                const int st = part ? j % kVStages : j % kKStages;
+                const uint32_t ph = (uint32_t)(part ? j / kVStages : j / kKStages) & 1u;
+                if (!warp_wait(part ? &sm.bar_vempty[st] : &sm.bar_kempty[st], ph ^ 1u, sm, P.status)) break;
+                uint8_t* tile = (part ? sm.v[st] : sm.k[st]) + (n & 3) * 4 * 1024;   // 8 rows: 1024 bytes of a panel
+                if (part) {
+                    const bool swap = g & 1;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const Scale2 s0 = scale2(__byte_perm(ss[i], 0, 0x4040)), s1 = scale2(__byte_perm(ss[i], 0, 0x4141));
+                        expand4(tile + i * 1024, voff, swap ? cc[i].y : cc[i].x, swap ? cc[i].x : cc[i].y,
+                                swap ? cc[i].w : cc[i].z, swap ? cc[i].z : cc[i].w, s0, s1);
+                    }
+                } else {
+                    const bool swap = t & 2;
+                    const uint32_t lo = swap ? 0x4141 : 0x4040, hi = swap ? 0x4040 : 0x4141;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const Scale2 s0 = scale2(__byte_perm(ss[i], 0, lo)), s1 = scale2(__byte_perm(ss[i], 0, hi));
+                        expand4(tile + i * 1024, koff, swap ? cc[i].z : cc[i].x, swap ? cc[i].w : cc[i].y,
+                                swap ? cc[i].x : cc[i].z, swap ? cc[i].y : cc[i].w, s0, s1);
+                    }
+                }
+                fence_proxy_async_smem();   // each lane's stores, before the arrival that covers them
+                __syncwarp();
+                if (lane == 0) mbar_arrive(part ? &sm.bar_vfull[st] : &sm.bar_kfull[st]);
+            }
+        } else {
+            if (any_bad && lane == 0) atomicOr(P.status, KVP_STATUS_MAP);
+            // ============================ MMA issuer ==========================
+            if (lane == 0) {
+                constexpr uint32_t idS = idesc_bf16(false);
+                constexpr uint32_t idO = idesc_bf16(true);
+                constexpr uint64_t kStageDesc = kTileBytes >> 4;
+                const uint64_t dq0 = sw128_desc(smem_u32(sm.q[0]), 16, 1024);
+                const uint64_t dq1 = sw128_desc(smem_u32(sm.q[1]), 16, 1024);
+                const uint64_t dk = sw128_desc(smem_u32(sm.k[0]), 16, 1024);
+                const uint64_t dv = sw128_desc(smem_u32(sm.v[0]), kPanel, 1024);
+                const uint32_t s0_tm = tmem, s1_tm = tmem + 128u, o0_tm = tmem + 256u, o1_tm = tmem + 384u;
+                bool ok = n_tiles > 0 && mbar_wait(&sm.bar_q[0], 0, sm, P.status);
+                if (ok && two) ok = mbar_wait(&sm.bar_q[1], 0, sm, P.status);
+                uint32_t ks = 0, kph = 0, vs = 0, vph = 0, pvs = 0;
+                bool k_known = false;
+                // While the first six MMAs of a GEMM are queued, the barriers of
+                // the next GEMM are tested without blocking.
+                for (int j = 0; ok && j < n_tiles; ++j) {
+                    if (!k_known && !(ok = mbar_wait(&sm.bar_kfull[ks], kph, sm, P.status))) break;
+                    tc_fence_after();
+                    const uint64_t kd = dk + ks * kStageDesc;
+                    const bool pv1 = two && j > 0;
+                    tc_gemm_ss_head(s0_tm, dq0, kd, idS);
+                    const bool pv1_ready = pv1 && mbar_test(&sm.bar_p_full[1], (uint32_t)(j - 1) & 1u);
+                    tc_gemm_ss_tail(s0_tm, dq0, kd, idS);
+                    tc_commit(&sm.bar_s_full[0]);
+                    if (pv1) {
+                        if (!pv1_ready && !(ok = mbar_wait(&sm.bar_p_full[1], (uint32_t)(j - 1) & 1u, sm, P.status))) break;
+                        tc_fence_after();
+                        const uint64_t vd = dv + pvs * kStageDesc;
+                        tc_gemm_ts_head(o1_tm, s1_tm, vd, idO, j > 1 ? 1u : 0u);
+                        tc_gemm_ts_tail(o1_tm, s1_tm, vd, idO);
+                    }
+                    bool pv0_ready = false;
+                    if (two) {
+                        tc_gemm_ss_head(s1_tm, dq1, kd, idS);
+                        pv0_ready = mbar_test(&sm.bar_vfull[vs], vph) && mbar_test(&sm.bar_p_full[0], (uint32_t)j & 1u);
+                        tc_gemm_ss_tail(s1_tm, dq1, kd, idS);
+                        tc_commit(&sm.bar_s_full[1]);
+                    }
+                    const uint32_t ks_n = ks + 1 == kKStages ? 0u : ks + 1;
+                    const uint32_t kph_n = ks + 1 == kKStages ? kph ^ 1u : kph;
+                    if (!pv0_ready && !(ok = mbar_wait(&sm.bar_vfull[vs], vph, sm, P.status) &&
+                                             mbar_wait(&sm.bar_p_full[0], (uint32_t)j & 1u, sm, P.status))) break;
+                    tc_fence_after();
+                    const uint64_t vd = dv + vs * kStageDesc;
+                    tc_gemm_ts_head(o0_tm, s0_tm, vd, idO, j > 0 ? 1u : 0u);
+                    k_known = j + 1 < n_tiles && mbar_test(&sm.bar_kfull[ks_n], kph_n);
+                    tc_gemm_ts_tail(o0_tm, s0_tm, vd, idO);
+                    pvs = vs;
+                    if (++vs == kVStages) { vs = 0; vph ^= 1u; }
+                    ks = ks_n;
+                    kph = kph_n;
+                }
+                if (ok) {
+                    tc_commit(&sm.bar_o_done[0]);
+                    if (two && mbar_wait(&sm.bar_p_full[1], (uint32_t)(n_tiles - 1) & 1u, sm, P.status)) {
+                        tc_fence_after();
+                        const uint64_t vd = dv + pvs * kStageDesc;
+                        tc_gemm_ts_head(o1_tm, s1_tm, vd, idO, n_tiles > 1 ? 1u : 0u);
+                        tc_gemm_ts_tail(o1_tm, s1_tm, vd, idO);
+                        tc_commit(&sm.bar_o_done[1]);
+                    }
+                }
+                // Drain: every issued MMA lands before TMEM is freed.
+                tc_commit(&sm.bar_mma_done);
+                const unsigned long long t0 = globaltimer();
+                while (!mbar_try_wait(&sm.bar_mma_done, 0) && globaltimer() - t0 < kWaitNs) {
+                }
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+        // ========================== softmax + epilogue ========================
+        const int qt = (warp - 4) >> 2;
+        const int row = (warp & 3) * 32 + lane;        // query row in tile == TMEM lane
+        const bool active = qt == 0 || two;            // this query tile has rows
+        Sees mine = {0, 0x7fffffff};                   // a row past the last takes every key (its Q is 0)
+        if (active) {
+            // Q: one row a thread; rows past the last are zero (never stored)
+            const int r = r0 + 128 * qt + row;
+            const uint4* src = reinterpret_cast<const uint4*>(q_row(P, b, h, min(r, rows - 1)));
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+                const uint4 y = r < rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(sm.q[qt] + (i >> 3) * kPanel + sw128_off(row, i & 7)) = y;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&sm.bar_q[qt]);
+            if (r < rows) mine = sees(P, start + r / P.group, end);
+        }
+        const uint32_t s_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u * qt;
+        const uint32_t o_tm = s_tm + 256u;
+        const float sl2 = P.scale_log2;
+        float m_run = -INFINITY, l_run = 0.f;          // m in log2 units
+        bool ok = true;
+        const int my_tiles = active ? n_tiles : 0;
+        for (int j = 0; j < my_tiles; ++j) {
+            if (!warp_wait(&sm.bar_s_full[qt], (uint32_t)j & 1u, sm, P.status)) { ok = false; break; }
+            tc_fence_after();
+            // S landing for the last query tile of a step means every MMA issued
+            // before has landed: K(j) and V(j-1) are no longer read.
+            if ((int)threadIdx.x == sm.releaser) {
+                mbar_arrive(&sm.bar_kempty[j % kKStages]);
+                if (j > 0) mbar_arrive(&sm.bar_vempty[(j - 1) % kVStages]);
+            }
+            // columns [0, sink) and [lo, hi) are visible
+            const int u = sm.u0 + j, pos = u < sm.na ? u : u - sm.na + sm.b0, key0 = pos * kBN;
+            int hi = mine.hi - key0;
+            if (sm.any_bad && page_of(s, sm.batch, pos) < 0) hi = 0;
+            const int sink = P.sink_rows - key0;
+            const int lo = mine.lo - key0 <= sink ? 0 : mine.lo - key0;
+            const bool masked = __any_sync(0xffffffffu, hi < kBN || (lo > 0 && sink < kBN));
+            if (masked) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < kBN; c0 += 32) {
+                    uint32_t y[32];
+                    KVP_TMEM_LD32(s_tm + c0, y);
+                    KVP_TMEM_WAIT_LD_DEP(y);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (c0 + c >= hi || (c0 + c < lo && c0 + c >= sink)) y[c] = 0xFF800000u;   // -inf
+                    KVP_TMEM_ST32(s_tm + c0, y);
+                }
+                tmem_wait_st();
+            }
+            uint32_t pk[64];
+            float rsum = 0.f, m_new = m_run;
+            const bool fresh = m_run == -INFINITY;     // no key seen yet
+            const bool skip = __all_sync(0xffffffffu, fresh);
+            // Exponentials against the running max; a row whose sum overgrows,
+            // or that has none yet, takes the tile's max and does them again.
+#pragma unroll 1
+            for (int attempt = skip ? 1 : 0;; ++attempt) {
+                if (attempt != 1 || !skip) {
+                    // (a row without keys keeps max -inf: subtract 0, every P is 0)
+                    const float mm = m_new == -INFINITY ? 0.f : m_new;
+                    // a hidden key's weight has to be 0: all of a masked tile on MUFU
+                    rsum = masked ? exp_row<false, 4, 0u>(s_tm, mm, sl2, kBN, pk)
+                                  : exp_row<false>(s_tm, mm, sl2, kBN, pk);
+                }
+                const bool redo = skip ? attempt == 1 : attempt == 0 && (fresh || !(rsum <= kRedoSum));
+                if (!__any_sync(0xffffffffu, redo)) break;
+                const float tmax = max_row<false>(s_tm, kBN);
+                if (redo) m_new = fmaxf(m_run, tmax * sl2);
+            }
+            const float alpha = m_new == m_run ? 1.f : ex2_approx(m_run - m_new);
+            l_run = l_run * alpha + rsum;
+            m_run = m_new;
+            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                // O_q holds PV_q(j-1) (complete: it was issued before S_q(j))
+#pragma unroll
+                for (int c4 = 0; c4 < 4; ++c4) {
+                    uint32_t o[32];
+                    KVP_TMEM_LD32(o_tm + 32 * c4, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                    KVP_TMEM_ST32(o_tm + 32 * c4, o);
+                }
+            }
+            // P (bf16: at most 2^-8 of each weight, without bias; the sum keeps
+            // 32 bits) -> the first 64 columns of S_q, key 2c in the low half
+            KVP_TMEM_ST32(s_tm, pk);
+            KVP_TMEM_ST32(s_tm + 32, (pk + 32));
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sm.bar_p_full[qt]);
+        }
+        const int r = sm.row0 + 128 * qt + row;
+        const bool mine_to_write = active && r < sm.rows;
+        if (ok && my_tiles > 0) ok = warp_wait(&sm.bar_o_done[qt], 0, sm, P.status);
+        tc_fence_after();
+        if (P.splits > 1) {
+            float2* ml = ws_ml(P, sm.batch, sm.head, r, sm.split);
+            float* dst = ws_o(P, sm.batch, sm.head, r, sm.split);
+            if (ok && mine_to_write) *ml = make_float2(m_run, l_run);   // (a split without pages: -inf, 0)
+#pragma unroll 1
+            for (int c0 = 0; ok && my_tiles > 0 && c0 < kKv4Head; c0 += 32) {
+                uint32_t o[32];
+                KVP_TMEM_LD32(o_tm + c0, o);
+                KVP_TMEM_WAIT_LD_DEP(o);
+                if (mine_to_write) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4)
+                        *reinterpret_cast<uint4*>(dst + c0 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                }
+                __syncwarp();
+            }
+        } else {
+            const float inv = l_run == 0.f ? 0.f : 1.f / l_run;         // a row without keys is 0
+            __nv_bfloat16* dst = out_row(P, sm.batch, sm.head, r);
+#pragma unroll 1
+            for (int c0 = 0; ok && my_tiles > 0 && c0 < kKv4Head; c0 += 32) {
+                uint32_t o[32];
+                KVP_TMEM_LD32(o_tm + c0, o);
+                KVP_TMEM_WAIT_LD_DEP(o);
+                if (mine_to_write) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8) {
+                        uint4 y;
+                        y.x = pack_bf16(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv);
+                        y.y = pack_bf16(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
+                        y.z = pack_bf16(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv);
+                        y.w = pack_bf16(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv);
+                        *reinterpret_cast<uint4*>(dst + c0 + c) = y;
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+}  // namespace
+
+int launch_kv4_tiles(const Kv4Params& P, unsigned grid, cudaStream_t stream) {
+    static PerDeviceOnce setup;
+    const int smem = (int)sizeof(Smem);
+    const int rc = setup([&](int dev) -> int {
+        int optin = 0;
+        KVP_CUDA(cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev));
+        if (smem > optin) {
+            set_error("attn_kv4: needs %d B of shared memory per block, device allows %d", smem, optin);
+            return KVP_ERR_UNSUPPORTED;
+        }
+        // setmaxnreg.inc waits until the warpgroup's registers exist in the
+        // CTA's pool: refuse a build whose launch pool is smaller than the split.
+        cudaFuncAttributes fa;
+        KVP_CUDA(cudaFuncGetAttributes(&fa, attn_kv4_sm100_kernel));
+        if ((long long)fa.numRegs * kThreads < (long long)kRegsLow * 128 + 2LL * kRegsHigh * 128) {
+            set_error("attn_kv4: kernel built with %d registers per thread, the register split needs %d",
+                      fa.numRegs, (kRegsLow * 128 + 2 * kRegsHigh * 128 + kThreads - 1) / kThreads);
+            return KVP_ERR_UNSUPPORTED;
+        }
+        KVP_CUDA(cudaFuncSetAttribute(attn_kv4_sm100_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        return KVP_OK;
+    });
+    if (rc != KVP_OK) return rc;
+    attn_kv4_sm100_kernel<<<grid, kThreads, smem, stream>>>(P);
+    KVP_CUDA(cudaGetLastError());
+    return KVP_OK;
+}
+
+}  // namespace kvp

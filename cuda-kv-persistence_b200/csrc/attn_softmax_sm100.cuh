@@ -81,9 +81,10 @@ __device__ __forceinline__ void ex2_poly2(float x0, float x1, float& y0, float& 
 // One S row's 32*kChunks columns from s_addr (this thread's TMEM lane) ->
 // P = 2^(s*sl2 - m) as packed bf16 pairs in pk, returns their fp32 sum.  Columns at or
 // past `left` are masked (-inf) when kMask.  One exponential in eight runs
-// on the FMA pipe (ex2_poly2), the rest on MUFU; scaling and the row sum use
-// f32x2 arithmetic.
-template <bool kMask, int kChunks = 4>
+// on the FMA pipe (ex2_poly2; the pairs of kPoly), the rest on MUFU, whose
+// 2^-inf is 0 where ex2_poly2's is not; scaling and the row sum use f32x2
+// arithmetic.
+template <bool kMask, int kChunks = 4, uint32_t kPoly = kPolyPairs>
 __device__ __forceinline__ float exp_row(uint32_t s_addr, float m, float sl2, int left,
                                          uint32_t (&pk)[16 * kChunks]) {
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
@@ -111,7 +112,7 @@ __device__ __forceinline__ float exp_row(uint32_t s_addr, float m, float sl2, in
             }
             float x0, x1, p0, p1;
             f2_unpack(f2_fma(f2_pack(s0, s1), sl2x2, negm2), x0, x1);
-            if ((kPolyPairs >> (c >> 1)) & 1u) {   // selected pairs on the FMA pipe
+            if ((kPoly >> (c >> 1)) & 1u) {   // selected pairs on the FMA pipe
                 ex2_poly2(x0, x1, p0, p1);
             } else {
                 p0 = ex2_approx(x0);
