@@ -321,33 +321,66 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
 }
 
 // ------------------------------------------------------------- joining splits
-// One warp per (sequence, K/V head, row), four dims a lane.  Launched while
-// the splits still run (programmatic stream serialization), so that its own
-// launch costs no time after them.
+// kJoin warps per (sequence, K/V head, row), four dims a lane; a warp adds
+// every kJoin-th split.  The lanes hold the splits' weights, so the partials'
+// loads wait for nothing but them.  Launched while the splits still run
+// (programmatic stream serialization), so that its own launch costs no time
+// after them.
+template <int kJoin>
 __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
+    __shared__ float4 part[8][32];
     const Kv4Span& s = P.span;
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % kJoin;
+    const long long w = (long long)blockIdx.x * (8 / kJoin) + warp / kJoin;
     cudaGridDependencySynchronize();                  // the partials are complete and visible
-    if (w >= (long long)s.batch * s.kv_heads * P.max_rows) return;
-    const int r = (int)(w % P.max_rows);
-    const int h = (int)(w / P.max_rows % s.kv_heads), b = (int)(w / P.max_rows / s.kv_heads);
-    int start, count;
-    if (!sequence(s, b, start, count) || r >= count * P.group) return;
-    const float2* ml = reinterpret_cast<const float2*>(P.ws_ml) + w * P.splits;
-    float top = -INFINITY;
-    for (int c = 0; c < P.splits; ++c) top = fmaxf(top, ml[c].x);
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < P.splits; ++c) {
-        const float2 y = ml[c];
-        if (y.y == 0.f) continue;                     // no key of this row
-        const float f = ex2(y.x - top);
-        sum += f * y.y;
-        const float4 o = reinterpret_cast<const float4*>(P.ws_o + (w * P.splits + c) * kKv4Head)[lane];
-        acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
+    int start, count, r = 0, h = 0, b = 0;
+    bool on = w < (long long)s.batch * s.kv_heads * P.max_rows;
+    if (on) {
+        r = (int)(w % P.max_rows);
+        h = (int)(w / P.max_rows % s.kv_heads);
+        b = (int)(w / P.max_rows / s.kv_heads);
+        on = sequence(s, b, start, count) && r < count * P.group;
     }
-    store_out(P, b, h, r, 4 * lane, acc, sum);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    if (on) {
+        const float2* ml = reinterpret_cast<const float2*>(P.ws_ml) + w * P.splits;
+        const float4* o = reinterpret_cast<const float4*>(P.ws_o + w * P.splits * kKv4Head) + lane;
+        float top = -INFINITY;
+        for (int c = lane; c < P.splits; c += 32) top = fmaxf(top, ml[c].x);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        for (int c0 = 0; c0 < P.splits; c0 += 32) {
+            float f = 0.f;                            // stays 0 for a split without keys of this row
+            if (c0 + lane < P.splits) {
+                const float2 y = ml[c0 + lane];
+                if (y.y != 0.f) f = ex2(y.x - top);
+                sum += f * y.y;
+            }
+            const int n = min(32, P.splits - c0);
+#pragma unroll 4
+            for (int c = sub; c < n; c += kJoin) {
+                const float g = __shfl_sync(0xffffffffu, f, c);
+                if (g != 0.f) {
+                    const float4 y = o[(long long)(c0 + c) * (kKv4Head / 4)];
+                    acc.x += g * y.x; acc.y += g * y.y; acc.z += g * y.z; acc.w += g * y.w;
+                }
+            }
+        }
+#pragma unroll
+        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    }
+    if (kJoin > 1) {
+        part[warp][lane] = acc;
+        __syncthreads();
+        if (sub) return;
+#pragma unroll
+        for (int c = 1; c < kJoin; ++c) {
+            const float4 y = part[warp + c][lane];
+            acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+        }
+    }
+    if (on) store_out(P, b, h, r, 4 * lane, acc, sum);
 }
 
 template <int NB>
@@ -447,17 +480,20 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
                              : launch_rows<2>(P, (unsigned)grid, stream);
     if (ws) {
         if (launched == KVP_OK) {
-            const long long warps = slots / P.splits;
+            const long long rows = slots / P.splits;
             cudaLaunchAttribute early;
             early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
             early.val.programmaticStreamSerializationAllowed = 1;
             cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3((unsigned)((warps + 7) / 8));
+            // a few splits: one warp a row; many: eight share them
+            const bool many = P.splits > 8;
+            cfg.gridDim = dim3((unsigned)(many ? rows : (rows + 7) / 8));
             cfg.blockDim = dim3(256);
             cfg.stream = stream;
             cfg.attrs = &early;
             cfg.numAttrs = 1;
-            const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel, P);
+            const cudaError_t e = many ? cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel<8>, P)
+                                       : cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel<1>, P);
             if (e != cudaSuccess) launched = cuda_status(e, "attn_kv4 join");
         }
         const cudaError_t e = cudaFreeAsync(ws, stream);
