@@ -73,12 +73,12 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     // CTA = (split, row tile, K/V head, sequence), split fastest
-    long long x = blockIdx.x;
-    const int split = (int)(x % P.splits);
-    x /= P.splits;
-    const int tile = (int)(x % P.row_tiles);
-    x /= P.row_tiles;
-    const int h = (int)(x % s.kv_heads), b = (int)(x / s.kv_heads);
+    uint32_t x = blockIdx.x;
+    const int split = (int)(x % (uint32_t)P.splits);
+    x /= (uint32_t)P.splits;
+    const int tile = (int)(x % (uint32_t)P.row_tiles);
+    x /= (uint32_t)P.row_tiles;
+    const int h = (int)(x % (uint32_t)s.kv_heads), b = (int)(x / (uint32_t)s.kv_heads);
     int start, count;
     cudaTriggerProgrammaticLaunchCompletion();        // the join may be launched; it waits for the data
     if (!sequence(s, b, start, count)) {
@@ -331,21 +331,21 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
     __shared__ float4 part[8][32];
     const Kv4Span& s = P.span;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % kJoin;
-    const long long w = (long long)blockIdx.x * (8 / kJoin) + warp / kJoin;
+    const uint32_t w = blockIdx.x * (8 / kJoin) + warp / kJoin, max_rows = (uint32_t)P.max_rows;
     cudaGridDependencySynchronize();                  // the partials are complete and visible
     int start, count, r = 0, h = 0, b = 0;
-    bool on = w < (long long)s.batch * s.kv_heads * P.max_rows;
+    bool on = w < (uint32_t)(s.batch * s.kv_heads) * max_rows;   // below 2^31: launch_attn_kv4
     if (on) {
-        r = (int)(w % P.max_rows);
-        h = (int)(w / P.max_rows % s.kv_heads);
-        b = (int)(w / P.max_rows / s.kv_heads);
+        r = (int)(w % max_rows);
+        h = (int)(w / max_rows % (uint32_t)s.kv_heads);
+        b = (int)(w / max_rows / (uint32_t)s.kv_heads);
         on = sequence(s, b, start, count) && r < count * P.group;
     }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
     if (on) {
-        const float2* ml = reinterpret_cast<const float2*>(P.ws_ml) + w * P.splits;
-        const float4* o = reinterpret_cast<const float4*>(P.ws_o + w * P.splits * kKv4Head) + lane;
+        const float2* ml = reinterpret_cast<const float2*>(P.ws_ml) + (long long)w * P.splits;
+        const float4* o = reinterpret_cast<const float4*>(P.ws_o + (long long)w * P.splits * kKv4Head) + lane;
         float top = -INFINITY;
         for (int c = lane; c < P.splits; c += 32) top = fmaxf(top, ml[c].x);
 #pragma unroll
@@ -461,6 +461,7 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
         const long long most = (keys + kKeys * kWarps - 1) / (kKeys * kWarps);
         P.splits = (int)std::max<long long>(1, std::min(std::min(want, most), 256LL));
     }
+    if ((long long)s.batch * s.kv_heads * P.max_rows > 0x7fffffffLL) P.splits = 1;   // the join counts rows in 31 bits
     const long long grid = units * P.splits;
     if (grid > 0x7fffffffLL) {
         set_error("attn_kv4: too many rows for one launch");

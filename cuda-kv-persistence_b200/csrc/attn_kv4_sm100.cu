@@ -58,8 +58,11 @@ struct __align__(1024) Smem {
     uint32_t tmem_base;
     int abort_flag;
     // the CTA's item, for what the softmax seldom needs (not held in registers)
-    volatile int batch, head, rows, row0, split, u0, na, b0, any_bad, releaser;
+    volatile int batch, head, rows, row0, split, u0, na, b0, any_bad, releaser, free0, free1;
 };
+
+// Bits [0, n) set.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // The four words and scale bytes of a lane's 16 bytes as four bf16 chunks.
 __device__ __forceinline__ void expand4(uint8_t* tile, const uint32_t (&off)[4], uint32_t w0, uint32_t w1,
@@ -82,13 +85,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // CTA = (split, query tile pair, K/V head, sequence), split fastest, last rows
     // (the longest spans) first
-    long long x = blockIdx.x;
-    const int split = (int)(x % P.splits);
-    x /= P.splits;
-    const int h = (int)(x % s.kv_heads);
-    x /= s.kv_heads;
-    const int b = (int)(x % s.batch);
-    const int r0 = (P.row_tiles - 1 - (int)(x / s.batch)) * 256;
+    uint32_t x = blockIdx.x;
+    const int split = (int)(x % (uint32_t)P.splits);
+    x /= (uint32_t)P.splits;
+    const int h = (int)(x % (uint32_t)s.kv_heads);
+    x /= (uint32_t)s.kv_heads;
+    const int b = (int)(x % (uint32_t)s.batch);
+    const int r0 = (P.row_tiles - 1 - (int)(x / (uint32_t)s.batch)) * 256;
     int start, count;
     if (!sequence(s, b, start, count)) {
         if (threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_MAP);
@@ -109,6 +112,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
         return u < na ? u : u - na + b0;
     };
     auto lookup = [&](int j) { return j < n_tiles ? page_of(s, b, page_pos(j)) : 0; };
+
+                    const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
+                    const uint8_t* head = static_cast<const uint8_t*>(s.pages) + h * kKv4PageHeadBytes;
+                    const int units = n_tiles * kUnits;
+                    uint4 c[4];
+                    uint32_t sc[4];
+                    auto load = [&](int n, int page) {
+                        const int part = (n >> 2) & 1;
+                        const uint8_t* p = head + (unsigned long long)(uint32_t)max(page, 0) * page_bytes +
+                                           (n & 3) * 4 * kKv4BlockBytes;
+                        const uint8_t* pc = p + (part ? kKv4VCode : 0) + lane * 16;
+                        const uint8_t* ps = p + (part ? kKv4VScale : kKv4KScale) + lane * 2;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            c[i] = *reinterpret_cast<const uint4*>(pc + i * kKv4BlockBytes);
+                            sc[i] = *reinterpret_cast<const uint16_t*>(ps + i * kKv4BlockBytes);
+                        }
+                    };
+                    // an expander's unit; its first is on its way while the CTA sets up
+    int n = warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : units;
+                    int page = lookup(n / kUnits), page1 = lookup((n + kExpanders) / kUnits);
+                    if (n < units) load(n, page);
 
     if (threadIdx.x == 0) {
         for (int q = 0; q < 2; ++q) {
@@ -136,6 +161,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
         sm.na = na;
         sm.b0 = b0;
         sm.any_bad = 0;
+        // the CTA's tiles that every row sees whole
+        sm.free0 = na + (last.lo + kBN - 1) / kBN - b0 - u0;
+        sm.free1 = na + first.hi / kBN - b0 - u0;
         sm.releaser = two ? 256 : 128;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async_smem();
@@ -150,7 +178,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
     tc_fence_before();
     const bool any_bad = __syncthreads_or(bad);   // some page is not in the pool: its keys are masked
     tc_fence_after();
-    if (any_bad) sm.any_bad = 1;                  // (every thread writes the same, its own reads follow)
+    if (any_bad) {                                // (every thread writes the same, its own reads follow)
+        sm.any_bad = 1;
+        sm.free1 = 0;
+    }
     const uint32_t tmem = sm.tmem_base;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
@@ -166,26 +197,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 voff[i] = (g >> 2) * kPanel + (2 * t + (i >> 1)) * 128 +
                           ((((g & 3) * 2) ^ (g & 1) ^ (2 * t) ^ (i >> 1) ^ (i & 1)) << 4);
             }
-            const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
-            const uint8_t* head = static_cast<const uint8_t*>(s.pages) + h * kKv4PageHeadBytes;
-            const int units = n_tiles * kUnits;
-            uint4 c[4];
-            uint32_t sc[4];
-            auto load = [&](int n, int page) {
-                const int part = (n >> 2) & 1;
-                const uint8_t* p = head + (unsigned long long)(uint32_t)max(page, 0) * page_bytes +
-                                   (n & 3) * 4 * kKv4BlockBytes;
-                const uint8_t* pc = p + (part ? kKv4VCode : 0) + lane * 16;
-                const uint8_t* ps = p + (part ? kKv4VScale : kKv4KScale) + lane * 2;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    c[i] = *reinterpret_cast<const uint4*>(pc + i * kKv4BlockBytes);
-                    sc[i] = *reinterpret_cast<const uint16_t*>(ps + i * kKv4BlockBytes);
-                }
-            };
-            int n = warp == 0 ? 0 : warp - 1;
-            int page = lookup(n / kUnits), page1 = lookup((n + kExpanders) / kUnits);
-            if (n < units) load(n, page);
             for (; n < units; n += kExpanders) {
                 page = page1;
                 page1 = lookup((n + 2 * kExpanders) / kUnits);
@@ -303,19 +314,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
         const int qt = (warp - 4) >> 2;
         const int row = (warp & 3) * 32 + lane;        // query row in tile == TMEM lane
         const bool active = qt == 0 || two;            // this query tile has rows
-        Sees mine = {0, 0x7fffffff};                   // a row past the last takes every key (its Q is 0)
+        // A row past the last (Q is 0, never stored) takes every key; a warp of
+        // such rows does no softmax.
+        Sees mine = {0, 0};
         if (active) {
-            // Q: one row a thread; rows past the last are zero (never stored)
-            const int r = r0 + 128 * qt + row;
-            const uint4* src = reinterpret_cast<const uint4*>(q_row(P, b, h, min(r, rows - 1)));
-#pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-                const uint4 y = r < rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(sm.q[qt] + (i >> 3) * kPanel + sw128_off(row, i & 7)) = y;
+            // Q: this warp's 32 rows, two rows a pass, 16 lanes on a row's 256 bytes;
+            // rows past the last are zero
+            const int rw = r0 + 128 * qt + (warp & 3) * 32, sub = lane >> 4, chunk = lane & 15;
+            int g = (rw + sub) % P.group;              // row r = i * group + g
+            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(P.attn.q) + b * P.attn.q_batch_stride +
+                                       (long long)((rw + sub) / P.group) * P.attn.q_row_stride +
+                                       (h * P.group + g) * kKv4Head + 8 * chunk;
+            const long long wrap = P.attn.q_row_stride - P.group * kKv4Head;
+            uint8_t* dst = sm.q[qt] + (chunk >> 3) * kPanel;
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+                const bool in = rw + sub + k < rows;
+                cp_async16(dst + sw128_off((warp & 3) * 32 + sub + k, chunk & 7), in ? src : P.attn.q, in ? 16u : 0u);
+                src += 2 * kKv4Head;
+                for (g += 2; g >= P.group; g -= P.group) src += wrap;
             }
+            cp_async_wait_all();
             fence_proxy_async_smem();
             mbar_arrive(&sm.bar_q[qt]);
-            if (r < rows) mine = sees(P, start + r / P.group, end);
+            if (rw + lane < rows) mine = sees(P, start + (rw + lane) / P.group, end);
+            else if (rw < rows) mine.hi = 0x7fffffff;
         }
         const uint32_t s_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u * qt;
         const uint32_t o_tm = s_tm + 256u;
@@ -332,30 +355,39 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 mbar_arrive(&sm.bar_kempty[j % kKStages]);
                 if (j > 0) mbar_arrive(&sm.bar_vempty[(j - 1) % kVStages]);
             }
-            // columns [0, sink) and [lo, hi) are visible
-            const int u = sm.u0 + j, pos = u < sm.na ? u : u - sm.na + sm.b0, key0 = pos * kBN;
-            int hi = mine.hi - key0;
-            if (sm.any_bad && page_of(s, sm.batch, pos) < 0) hi = 0;
-            const int sink = P.sink_rows - key0;
-            const int lo = mine.lo - key0 <= sink ? 0 : mine.lo - key0;
-            const bool masked = __any_sync(0xffffffffu, hi < kBN || (lo > 0 && sink < kBN));
+            if (__all_sync(0xffffffffu, mine.hi == 0)) {   // no row: what P's columns hold is never stored
+                tc_fence_before();
+                mbar_arrive(&sm.bar_p_full[qt]);
+                continue;
+            }
+            uint32_t pk[64];
+            float rsum = 0.f, m_new = m_run;
+            bool masked = j < sm.free0 || j >= sm.free1, none = masked;
             if (masked) {
+                // columns [0, sink) and [lo, hi) are visible
+                const int u = sm.u0 + j, pos = u < sm.na ? u : u - sm.na + sm.b0, key0 = pos * kBN;
+                int hi = mine.hi - key0;
+                if (sm.any_bad && page_of(s, sm.batch, pos) < 0) hi = 0;
+                const int sink = P.sink_rows - key0, lo = mine.lo - key0;
+                masked = false;
 #pragma unroll 1
                 for (int c0 = 0; c0 < kBN; c0 += 32) {
+                    const uint32_t vis = below(hi - c0) & (~below(lo - c0) | below(sink - c0));
+                    if (__any_sync(0xffffffffu, vis != 0u)) none = false;
+                    if (__all_sync(0xffffffffu, vis == 0xffffffffu)) continue;
+                    masked = true;
                     uint32_t y[32];
                     KVP_TMEM_LD32(s_tm + c0, y);
                     KVP_TMEM_WAIT_LD_DEP(y);
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
-                        if (c0 + c >= hi || (c0 + c < lo && c0 + c >= sink)) y[c] = 0xFF800000u;   // -inf
+                        if (!(vis >> c & 1u)) y[c] = 0xFF800000u;   // -inf
                     KVP_TMEM_ST32(s_tm + c0, y);
                 }
                 tmem_wait_st();
             }
-            uint32_t pk[64];
-            float rsum = 0.f, m_new = m_run;
             const bool fresh = m_run == -INFINITY;     // no key seen yet
-            const bool skip = __all_sync(0xffffffffu, fresh);
+            const bool skip = !none && __all_sync(0xffffffffu, fresh);
             // Exponentials against the running max; a row whose sum overgrows,
             // or that has none yet, takes the tile's max and does them again.
 #pragma unroll 1
@@ -367,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                     rsum = masked ? exp_row<false, 4, 0u>(s_tm, mm, sl2, kBN, pk)
                                   : exp_row<false>(s_tm, mm, sl2, kBN, pk);
                 }
-                const bool redo = skip ? attempt == 1 : attempt == 0 && (fresh || !(rsum <= kRedoSum));
+                const bool redo = skip ? attempt == 1 : attempt == 0 && !none && (fresh || !(rsum <= kRedoSum));
                 if (!__any_sync(0xffffffffu, redo)) break;
                 const float tmax = max_row<false>(s_tm, kBN);
                 if (redo) m_new = fmaxf(m_run, tmax * sl2);
@@ -396,47 +428,63 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             tc_fence_before();
             mbar_arrive(&sm.bar_p_full[qt]);
         }
-        const int r = sm.row0 + 128 * qt + row;
-        const bool mine_to_write = active && r < sm.rows;
+        // A warp's rows go out through its own rows of the Q tile (every S
+        // has landed): a row's 128 bytes by eight lanes, four rows a store.
+        const int eb = sm.batch, eh = sm.head, es = sm.split, er = sm.rows, r = sm.row0 + 128 * qt + row;
         if (ok && my_tiles > 0) ok = warp_wait(&sm.bar_o_done[qt], 0, sm, P.status);
         tc_fence_after();
-        if (P.splits > 1) {
-            float2* ml = ws_ml(P, sm.batch, sm.head, r, sm.split);
-            float* dst = ws_o(P, sm.batch, sm.head, r, sm.split);
-            if (ok && mine_to_write) *ml = make_float2(m_run, l_run);   // (a split without pages: -inf, 0)
+        uint8_t* stage = sm.q[qt] + (warp & 3) * 32 * 128;
+        const int rw = r - lane, sub = lane >> 3, chunk = lane & 7;
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;         // a row without keys is 0
+        if (P.splits > 1 && ok && active && r < er)                 // (a split without pages: -inf, 0)
+            *ws_ml(P, eb, eh, r, es) = make_float2(m_run, l_run);
+        // row rw + sub + 4 i of the workspace (rows splits * 512 bytes apart) or of the output
+        uint8_t* ws = P.splits > 1 ? reinterpret_cast<uint8_t*>(ws_o(P, eb, eh, rw + sub, es)) + 16 * chunk : nullptr;
+        const long long ws_step = 4LL * P.splits * kKv4Head * 4;
+        uint8_t* out = reinterpret_cast<uint8_t*>(static_cast<__nv_bfloat16*>(P.attn.out) + eb * P.attn.out_batch_stride +
+                                                  (long long)eh * P.group * kKv4Head) + 16 * chunk;
+        const int step = P.splits > 1 ? 32 : 64;                    // dims that make 128 bytes
 #pragma unroll 1
-            for (int c0 = 0; ok && my_tiles > 0 && c0 < kKv4Head; c0 += 32) {
-                uint32_t o[32];
-                KVP_TMEM_LD32(o_tm + c0, o);
-                KVP_TMEM_WAIT_LD_DEP(o);
-                if (mine_to_write) {
+        for (int c0 = 0; ok && my_tiles > 0 && c0 < kKv4Head; c0 += step) {
+            uint32_t o[32];
+            KVP_TMEM_LD32(o_tm + c0, o);
+            KVP_TMEM_WAIT_LD_DEP(o);
+            if (P.splits > 1) {
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4)
-                        *reinterpret_cast<uint4*>(dst + c0 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-                }
-                __syncwarp();
-            }
-        } else {
-            const float inv = l_run == 0.f ? 0.f : 1.f / l_run;         // a row without keys is 0
-            __nv_bfloat16* dst = out_row(P, sm.batch, sm.head, r);
+                for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                        make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            } else {
 #pragma unroll 1
-            for (int c0 = 0; ok && my_tiles > 0 && c0 < kKv4Head; c0 += 32) {
-                uint32_t o[32];
-                KVP_TMEM_LD32(o_tm + c0, o);
-                KVP_TMEM_WAIT_LD_DEP(o);
-                if (mine_to_write) {
+                for (int e = 0; e < 2; ++e) {
+                    if (e) {
+                        KVP_TMEM_LD32(o_tm + c0 + 32, o);
+                        KVP_TMEM_WAIT_LD_DEP(o);
+                    }
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
+                    for (int c = 0; c < 4; ++c) {
                         uint4 y;
-                        y.x = pack_bf16(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv);
-                        y.y = pack_bf16(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
-                        y.z = pack_bf16(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv);
-                        y.w = pack_bf16(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv);
-                        *reinterpret_cast<uint4*>(dst + c0 + c) = y;
+                        y.x = pack_bf16(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv);
+                        y.y = pack_bf16(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv);
+                        y.z = pack_bf16(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv);
+                        y.w = pack_bf16(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv);
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * e + c) ^ (lane & 7)) << 4)) = y;
                     }
                 }
-                __syncwarp();
             }
+            __syncwarp();
+            int qi = (rw + sub) / P.group, qg = (rw + sub) % P.group;   // row = qi * group + qg
+#pragma unroll 4
+            for (int i = 0; i < 8; ++i) {
+                const int k = 4 * i + sub;
+                const uint4 y = *reinterpret_cast<const uint4*>(stage + k * 128 + ((chunk ^ (k & 7)) << 4));
+                uint8_t* dst = P.splits > 1 ? ws + i * ws_step + c0 * 4
+                                            : out + (qi * P.attn.out_row_stride + qg * kKv4Head + c0) * 2;
+                if (rw + k < er) *reinterpret_cast<uint4*>(dst) = y;
+                if (P.splits == 1)
+                    for (qg += 4; qg >= P.group; qg -= P.group) ++qi;
+            }
+            __syncwarp();
         }
     }
     tc_fence_before();
