@@ -62,7 +62,30 @@ template <int NB>
 struct RowsSmem {
     float o[kWarps][8 * NB][kKv4Head];
     float m[kWarps][8 * NB], l[kWarps][8 * NB];
+    float jo[8 * NB][kKv4Head];                // the CTA's partial, read by its cluster
+    float jm[8 * NB], jl[8 * NB];
 };
+
+// Shared memory of another CTA of the cluster.
+__device__ __forceinline__ uint32_t peer(const void* p, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float peer_f(const float* p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer(p, rank)));
+    return v;
+}
+__device__ __forceinline__ float4 peer_f4(const float* p, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer(p, rank)));
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // NB blocks of 8 query rows.
 template <int NB>
@@ -316,8 +339,40 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
             const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][q][d]);
             acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
         }
-        put(P, b, h, r, split, d, acc, top, sum);
+        if (P.cluster) {
+            *reinterpret_cast<float4*>(&sm.jo[q][d]) = acc;
+            if (d == 0) {
+                sm.jm[q] = top;
+                sm.jl[q] = sum;
+            }
+        } else {
+            put(P, b, h, r, split, d, acc, top, sum);
+        }
     }
+    if (!P.cluster) return;
+    // The splits are a cluster: each CTA joins its share of the rows' dims from
+    // all of them, out of their shared memory.
+    cluster_sync();
+    const int items = 8 * NB * (kKv4Head / 4), share = (items + P.splits - 1) / P.splits;
+    for (int e = split * share + threadIdx.x; e < min(items, (split + 1) * share); e += kDecThreads) {
+        const int q = e / (kKv4Head / 4), d = e % (kKv4Head / 4) * 4;
+        const int r = r0 + q;
+        if (r >= rows) continue;
+        float top = -INFINITY;
+        for (int c = 0; c < P.splits; ++c) top = fmaxf(top, peer_f(&sm.jm[q], c));
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = 0; c < P.splits; ++c) {
+            const float l1 = peer_f(&sm.jl[q], c), m1 = peer_f(&sm.jm[q], c);
+            const float4 y = peer_f4(&sm.jo[q][d], c);
+            const float f = l1 == 0.f ? 0.f : ex2(m1 - top);   // (no key of this row: O is 0)
+            sum += f * l1;
+            acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
+        }
+        store_out(P, b, h, r, d, acc, sum);
+    }
+    cluster_sync();                            // nobody leaves while its memory is read
 }
 
 // ------------------------------------------------------------- joining splits
@@ -384,16 +439,62 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
 }
 
 template <int NB>
-int launch_rows(const Kv4Params& P, unsigned grid, cudaStream_t stream) {
+cudaLaunchConfig_t rows_config(unsigned grid, int cluster, cudaLaunchAttribute* attr, cudaStream_t stream) {
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = (unsigned)cluster;
+    attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kDecThreads);
+    cfg.dynamicSmemBytes = sizeof(RowsSmem<NB>);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cfg;
+}
+
+constexpr int kMaxCluster = 8;
+
+// What a device runs at once: CTAs of the rows kernel, clusters of 2, 4 and 8
+// of them (slot i: 2^i CTAs).  Asked once per device.
+struct RowsFit {
+    int at_once[PerDeviceOnce::kMaxDevices][4];
+};
+template <int NB>
+int rows_fit(const int** at_once) {
     static PerDeviceOnce setup;
-    const int rc = setup([](int) -> int {
+    static RowsFit fit;
+    const int rc = setup([](int dev) -> int {
         KVP_CUDA(cudaFuncSetAttribute(attn_kv4_rows_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)sizeof(RowsSmem<NB>)));
+        for (int i = 0; i < 4; ++i) {
+            cudaLaunchAttribute attr;
+            const cudaLaunchConfig_t cfg = rows_config<NB>(1024, 1 << i, &attr, nullptr);
+            int n = 0;
+            if (i == 0) {
+                int sms = 0;
+                KVP_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_kv4_rows_kernel<NB>, kDecThreads,
+                                                                       sizeof(RowsSmem<NB>)));
+                KVP_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+                n *= sms;
+            } else {
+                KVP_CUDA(cudaOccupancyMaxActiveClusters(&n, attn_kv4_rows_kernel<NB>, &cfg));
+            }
+            fit.at_once[dev][i] = n;
+        }
         return KVP_OK;
     });
-    if (rc != KVP_OK) return rc;
-    attn_kv4_rows_kernel<NB><<<grid, kDecThreads, sizeof(RowsSmem<NB>), stream>>>(P);
-    KVP_CUDA(cudaGetLastError());
+    int dev = 0;
+    if (rc == KVP_OK) KVP_CUDA(cudaGetDevice(&dev));
+    *at_once = fit.at_once[dev];
+    return rc;
+}
+
+template <int NB>
+int launch_rows(const Kv4Params& P, unsigned grid, cudaStream_t stream) {
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = rows_config<NB>(grid, P.cluster ? P.splits : 1, &attr, stream);
+    KVP_CUDA(cudaLaunchKernelEx(&cfg, attn_kv4_rows_kernel<NB>, P));
     return KVP_OK;
 }
 
@@ -450,16 +551,28 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
         const long long span = (long long)(tile_rows / P.group + 2 + (long long)a.tokens) + P.window_rows + P.sink_rows;
         keys = std::min(keys, span);
     }
-    const int sms = sm_count();
     if (tiles) {
-        P.splits = tile_splits(units, (int)((keys + kKv4PageRows - 1) / kKv4PageRows), sms);
+        P.splits = tile_splits(units, (int)((keys + kKv4PageRows - 1) / kKv4PageRows), sm_count());
     } else {
-        // As many splits as fill two CTAs an SM (one more CTA would wait for a
-        // second round: 37 us against 25 at 32768 keys x 12 heads), a step for
-        // each warp of a split at least.
-        const long long want = 2LL * sms / units;
-        const long long most = (keys + kKeys * kWarps - 1) / (kKeys * kWarps);
-        P.splits = (int)std::max<long long>(1, std::min(std::min(want, most), 256LL));
+        const int* at_once = nullptr;
+        const int rf = nb == 1 ? rows_fit<1>(&at_once) : rows_fit<2>(&at_once);
+        if (rf != KVP_OK) return rf;
+        // As many splits as the device runs at once (one more CTA would wait for
+        // a second round: 37 us against 25 at 32768 keys x 12 heads), with a
+        // step for each warp of a split at least.
+        const long long steps = (keys + kKeys - 1) / kKeys;
+        const long long want = std::max<long long>(1, std::min(std::min(at_once[0] / units, (steps + kWarps - 1) / kWarps), 256LL));
+        // Splits that are a cluster join without workspace and second launch,
+        // which is worth two steps more a warp (4099 keys x 12 heads: 8 in a
+        // cluster 8.2 us at 10 us of host time, 12 and a join 8.0 at 14;
+        // 16 sequences of 8191 x 8 heads: 2 in a cluster 34.4, 2 and a join
+        // 36.3; 32768 x 12 heads: 8 in a cluster 27.2, 24 and a join 20.0).
+        auto a_warp = [&](long long c) { return (steps + c * kWarps - 1) / (c * kWarps); };
+        int c = 0;
+        for (int i = 3; i > 0 && !c; --i)
+            if ((1 << i) <= want && units <= at_once[i]) c = 1 << i;
+        P.cluster = c > 0 && a_warp(c) <= a_warp(want) + 2;
+        P.splits = P.cluster ? c : (int)want;
     }
     if ((long long)s.batch * s.kv_heads * P.max_rows > 0x7fffffffLL) P.splits = 1;   // the join counts rows in 31 bits
     const long long grid = units * P.splits;
@@ -469,7 +582,7 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     }
     const long long slots = (long long)s.batch * s.kv_heads * P.max_rows * P.splits;
     void* ws = nullptr;
-    if (P.splits > 1) {
+    if (P.splits > 1 && !P.cluster) {
         cudaMemPool_t pool = nullptr;
         KVP_CUDA(workspace_pool(&pool));
         KVP_CUDA(cudaMallocFromPoolAsync(&ws, (size_t)slots * (kKv4Head + 2) * sizeof(float), pool, stream));

@@ -18,6 +18,7 @@ struct Kv4Params {
     int sink_rows;           // sinks * tokens, at most the capacity
     int group, max_rows;     // query heads per K/V head; rows * group
     int tokens, row_tiles, splits;
+    int cluster;             // the splits of a row tile are one cluster and join by themselves
     float scale_log2;        // log2(e) / sqrt(128)
     float rise;              // kRise in score units
 };

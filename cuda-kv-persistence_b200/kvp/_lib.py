@@ -173,9 +173,9 @@ SIGNATURES = {
     "kvp_layernorm_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_longlong,
                                      C.c_int, C.c_float, C.c_void_p]),
     "kvp_kv4_page_bytes": (C.c_longlong, [C.c_int]),
-    "kvp_kv4_write": (C.c_int, [C.POINTER(Kv4Span), C.POINTER(Kv4Rows), C.c_void_p]),
-    "kvp_kv4_read": (C.c_int, [C.POINTER(Kv4Span), C.POINTER(Kv4Rows), C.c_void_p]),
-    "kvp_attn_kv4": (C.c_int, [C.POINTER(Kv4Span), C.POINTER(Kv4Attn), C.c_void_p]),
+    "kvp_kv4_write": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kvp_kv4_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kvp_attn_kv4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "kvp_session_plan_stack": (C.c_int, [C.c_void_p, C.c_void_p]),
     "kvp_session_finish": (C.c_int, [C.c_void_p]),
     "kvp_session_info": (C.c_int, [C.c_void_p, C.POINTER(StepInfo)]),

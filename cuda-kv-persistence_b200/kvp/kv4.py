@@ -20,11 +20,11 @@ Everything is queued on the current stream of the tensors' device, or on
 
 from __future__ import annotations
 
-from ctypes import byref
+import struct
 
 import torch
 
-from ._lib import Kv4Attn, Kv4Rows, Kv4Span, KvpError, check, lib
+from ._lib import KvpError, check, lib
 
 PAGE_ROWS = 128
 PAGE_HEAD_BYTES = 18432
@@ -32,6 +32,14 @@ PAGE_HEAD_BYTES = 18432
 _ROW_TYPES = (torch.bfloat16, torch.float32)
 _Q_TYPES = (torch.bfloat16,)
 _MAX_INT = 2 ** 31
+# kvp_kv4_span, kvp_kv4_rows and kvp_kv4_attn in native layout (a packed
+# bytes object costs a fifth of a filled ctypes structure)
+_SPAN = struct.Struct("@PPPPqiiiii4x").pack
+_ROWS = struct.Struct("@PPqqi4x").pack
+_ATTN = struct.Struct("@PPqqqqiiii").pack
+# the current stream's handle without building a Stream object
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def alloc_pages(n_pages: int, kv_heads: int, device="cuda"):
@@ -66,24 +74,21 @@ def _rows3(t, name: str, dtypes, heads: int):
 def _pool(pages):
     """(n_pages, kv_heads) of a pool."""
     shape = pages.shape
-    if pages.dtype != torch.uint8 or len(shape) != 3 or shape[2] != PAGE_HEAD_BYTES or \
+    if len(shape) != 3 or shape[2] != PAGE_HEAD_BYTES or pages.dtype != torch.uint8 or \
             not pages.is_contiguous():
         _bad(f"pages must be a contiguous uint8 [n_pages, kv_heads, {PAGE_HEAD_BYTES}] tensor")
     return shape[0], shape[1]
 
 
-def _batch_ints(t, name: str, batch: int, dev: int) -> int:
-    if t is None:
-        return 0
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != batch or not t.is_contiguous():
-        _bad(f"{name} must be a contiguous int32 [{batch}] tensor")
+def _ints(t, name: str, batch: int, dev: int, dims: int) -> int:
+    if t.dtype != torch.int32 or t.dim() != dims or t.shape[0] != batch or not t.is_contiguous():
+        _bad(f"{name} must be a contiguous int32 [{batch}{', pages' if dims == 2 else ''}] tensor")
     if t.get_device() != dev:
         _bad(f"tensors on {t.device} and cuda:{dev}")
     return t.data_ptr()
 
 
-def _span(pages, batch: int, rows: int, page_map, start: int, starts, counts, a, b):
-    n_pages, kv_heads = pages.shape[0], pages.shape[1]
+def _span(pages, n_pages, kv_heads, batch: int, rows: int, page_map, start: int, starts, counts, a, b):
     dev = pages.get_device()
     if dev < 0:
         _bad("pages must be a CUDA tensor")
@@ -93,27 +98,22 @@ def _span(pages, batch: int, rows: int, page_map, start: int, starts, counts, a,
     if page_map is None:
         stride, map_ptr = n_pages // max(batch, 1), 0
     else:
-        if page_map.dtype != torch.int32 or page_map.dim() != 2 or page_map.shape[0] != batch or \
-                not page_map.is_contiguous():
-            _bad(f"page_map must be a contiguous int32 [{batch}, pages] tensor")
-        if page_map.get_device() != dev:
-            _bad(f"tensors on {page_map.device} and cuda:{dev}")
-        stride, map_ptr = page_map.shape[1], page_map.data_ptr()
-    if not (0 <= start < _MAX_INT and rows < _MAX_INT and stride < _MAX_INT):
-        _bad(f"start {start}, rows {rows} or {stride} pages out of range")
-    return Kv4Span(pages.data_ptr(), map_ptr, _batch_ints(starts, "starts", batch, dev),
-                   _batch_ints(counts, "counts", batch, dev), n_pages, kv_heads, batch, stride, start, rows)
+        map_ptr = _ints(page_map, "page_map", batch, dev, 2)
+        stride = page_map.shape[1]
+    if not (0 <= start < _MAX_INT and rows < _MAX_INT and stride < _MAX_INT and batch < _MAX_INT):
+        _bad(f"start {start}, rows {rows}, batch {batch} or {stride} pages out of range")
+    return dev, _SPAN(pages.data_ptr(), map_ptr,
+                      0 if starts is None else _ints(starts, "starts", batch, dev, 1),
+                      0 if counts is None else _ints(counts, "counts", batch, dev, 1),
+                      n_pages, kv_heads, batch, stride, start, rows)
 
 
-def _call(fn, what, pages, stream, *args):
-    dev = pages.get_device()
-    if stream is None:
-        stream = torch.cuda.current_stream(dev).cuda_stream
+def _call(fn, what, dev, stream, span, args):
     if dev == torch.cuda.current_device():
-        rc = fn(*args, stream)
+        rc = fn(span, args, _raw_stream(dev) if stream is None else stream)
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, stream)
+            rc = fn(span, args, _raw_stream(dev) if stream is None else stream)
     if rc < 0:
         check(rc, what)
 
@@ -122,14 +122,14 @@ def _kv(pages, k, v, page_map, start, starts, counts):
     some = k if k is not None else v
     if some is None:
         _bad("no rows")
-    heads = _pool(pages)[1]
+    n_pages, heads = _pool(pages)
     b, n, rs, bs = shape = _rows3(some, "k" if k is not None else "v", _ROW_TYPES, heads)
     if k is not None and v is not None and (_rows3(v, "v", _ROW_TYPES, heads) != shape or
                                             k.dtype != v.dtype):
         _bad("k and v must agree in shape, strides and type")
-    span = _span(pages, b, n, page_map, start, starts, counts, k, v)
-    return span, Kv4Rows(0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), rs, bs,
-                         some.element_size())
+    dev, span = _span(pages, n_pages, heads, b, n, page_map, start, starts, counts, k, v)
+    return dev, span, _ROWS(0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), rs, bs,
+                            some.element_size())
 
 
 def write(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=None,
@@ -137,15 +137,15 @@ def write(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=Non
     """Quantises rows k, v (bf16 or fp32) into the cache."""
     if k is None or v is None:
         _bad("write needs k and v")
-    span, rows = _kv(pages, k, v, page_map, start, starts, counts)
-    _call(lib().kvp_kv4_write, "kvp_kv4_write", pages, stream, byref(span), byref(rows))
+    dev, span, rows = _kv(pages, k, v, page_map, start, starts, counts)
+    _call(lib().kvp_kv4_write, "kvp_kv4_write", dev, stream, span, rows)
 
 
 def read(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=None,
          stream=None) -> None:
     """Fills k and v (bf16 or fp32; either may be None) with the rows' values."""
-    span, rows = _kv(pages, k, v, page_map, start, starts, counts)
-    _call(lib().kvp_kv4_read, "kvp_kv4_read", pages, stream, byref(span), byref(rows))
+    dev, span, rows = _kv(pages, k, v, page_map, start, starts, counts)
+    _call(lib().kvp_kv4_read, "kvp_kv4_read", dev, stream, span, rows)
 
 
 def attn(q, pages, out, *, heads: int, page_map=None, start: int = 0, starts=None, counts=None,
@@ -154,11 +154,13 @@ def attn(q, pages, out, *, heads: int, page_map=None, start: int = 0, starts=Non
     position p, in frame f = p // tokens, sees the cached rows up to the end of
     its frame (and of this call's rows) that lie in the last `window` frames (0: all) or the
     first `sinks` frames.  The call's own rows are keys: write them first."""
-    _pool(pages)
+    n_pages, kv_heads = _pool(pages)
     b, n, qr, qb = _rows3(q, "q", _Q_TYPES, heads)
     ob, on, orow, obatch = _rows3(out, "out", _Q_TYPES, heads)
     if ob != b or on != n:
         _bad("q and out must agree in shape")
-    span = _span(pages, b, n, page_map, start, starts, counts, q, out)
-    a = Kv4Attn(q.data_ptr(), out.data_ptr(), qr, qb, orow, obatch, heads, tokens, window, sinks)
-    _call(lib().kvp_attn_kv4, "kvp_attn_kv4", pages, stream, byref(span), byref(a))
+    dev, span = _span(pages, n_pages, kv_heads, b, n, page_map, start, starts, counts, q, out)
+    if not (0 < tokens < _MAX_INT and 0 <= window < _MAX_INT and 0 <= sinks < _MAX_INT):
+        _bad(f"tokens {tokens}, window {window} or sinks {sinks} out of range")
+    _call(lib().kvp_attn_kv4, "kvp_attn_kv4", dev, stream, span,
+          _ATTN(q.data_ptr(), out.data_ptr(), qr, qb, orow, obatch, heads, tokens, window, sinks))

@@ -168,3 +168,14 @@ def test_oracle_attention_is_softmax():
             w = np.exp(s - s.max())
             assert np.allclose(out[r, h], w @ v[: r + 1, h // 2] / w.sum(), atol=1e-12)
     assert np.all(tol >= 0)
+
+
+def test_packed_arguments_are_the_c_structures():
+    """kvp.kv4 packs its arguments; the layouts are those of include/kvp.h."""
+    from kvp import kv4
+    s = Kv4Span(1, 2, 3, 4, 5, 6, 7, 8, 9, 10)
+    assert kv4._SPAN(1, 2, 3, 4, 5, 6, 7, 8, 9, 10) == bytes(s)
+    r = Kv4Rows(1, 2, 3, 4, 5)
+    assert kv4._ROWS(1, 2, 3, 4, 5) == bytes(r)
+    a = Kv4Attn(1, 2, 3, 4, 5, 6, 7, 8, 9, 10)
+    assert kv4._ATTN(1, 2, 3, 4, 5, 6, 7, 8, 9, 10) == bytes(a)
