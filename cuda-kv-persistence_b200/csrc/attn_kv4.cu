@@ -561,7 +561,10 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
         // a second round: 37 us against 25 at 32768 keys x 12 heads), with a
         // step for each warp of a split at least.
         const long long steps = (keys + kKeys - 1) / kKeys;
-        const long long want = std::max<long long>(1, std::min(std::min(at_once[0] / units, (steps + kWarps - 1) / kWarps), 256LL));
+        // Beyond 32 of them two steps for each warp: a long join costs more than
+        // it saves (60000 keys of one head: 48 splits 13.4 us, 235 17.3).
+        const long long most = std::max(std::min(32LL, (steps + kWarps - 1) / kWarps), steps / (4 * kWarps));
+        const long long want = std::max<long long>(1, std::min(at_once[0] / units, most));
         // Splits that are a cluster join without workspace and second launch,
         // which is worth two steps more a warp (4099 keys x 12 heads: 8 in a
         // cluster 8.2 us at 10 us of host time, 12 and a join 8.0 at 14;

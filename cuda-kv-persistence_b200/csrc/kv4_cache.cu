@@ -46,19 +46,40 @@ __device__ __forceinline__ bool item_of(const Kv4Span& s, long long w, int block
     return true;
 }
 
-// 16 values as bf16 pairs, from bf16 or fp32 (rounded to bf16 first).
+// 16 bf16 values, two to a register.
 __device__ __forceinline__ void load16(const __nv_bfloat16* p, uint32_t (&x)[8]) {
     const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 8);
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
-__device__ __forceinline__ void load16(const float* p, uint32_t (&x)[8]) {
+
+// fp32 rows are twice as long: a lane's 64 or 128 bytes of a row no longer
+// stay in L1 between its loads (3.4 TB/s), so they come in whole rows, 16
+// bytes a lane, and go as bf16 through shared memory, [8 rows][16 chunks of
+// 16 bytes], the chunks swapped so that neither way of reading conflicts.
+__device__ __forceinline__ int stage_at(int row, int chunk) {
+    return row * 256 + ((chunk ^ (chunk >> 3 & 1) ^ (row & 1) << 1 ^ (row >> 1 & 1) << 2 ^ (row >> 2 & 1)) << 4);
+}
+__device__ __forceinline__ void load16(const uint8_t* stage, int row, int chunk, uint32_t (&x)[8]) {
+    const uint4 a = *reinterpret_cast<const uint4*>(stage + stage_at(row, chunk));
+    const uint4 b = *reinterpret_cast<const uint4*>(stage + stage_at(row, chunk + 1));
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void fetch_rows(float4 (&y)[kKv4BlockRows], const float* p, long long row_stride, int first,
+                                           int count, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float4 a = *reinterpret_cast<const float4*>(p + 4 * i);
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(a.x, a.y), hi = __floats2bfloat162_rn(a.z, a.w);
-        x[2 * i] = reinterpret_cast<const uint32_t&>(lo);
-        x[2 * i + 1] = reinterpret_cast<const uint32_t&>(hi);
+    for (int r = 0; r < kKv4BlockRows; ++r)
+        y[r] = first + r >= 0 && first + r < count
+                   ? __ldcs(reinterpret_cast<const float4*>(p + (first + r) * row_stride + 4 * lane))
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ void stage_rows(uint8_t* stage, const float4 (&y)[kKv4BlockRows], int lane) {
+#pragma unroll
+    for (int r = 0; r < kKv4BlockRows; ++r) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(y[r].x, y[r].y), hi = __floats2bfloat162_rn(y[r].z, y[r].w);
+        *reinterpret_cast<uint2*>(stage + stage_at(r, lane >> 1) + (lane & 1) * 8) =
+            make_uint2(reinterpret_cast<const uint32_t&>(lo), reinterpret_cast<const uint32_t&>(hi));
     }
 }
 
@@ -111,10 +132,11 @@ __device__ __forceinline__ uint32_t quantise16(uint32_t (&x)[8], uint32_t (&word
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) kv4_write_kernel(const Kv4Span s, const T* __restrict__ k,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) kv4_write_kernel(const Kv4Span s, const T* __restrict__ k,
                                                              const T* __restrict__ v, long long row_stride,
                                                              long long batch_stride, int blocks,
                                                              long long items, int* status) {
+    __shared__ __align__(16) uint8_t stage[sizeof(T) == 4 ? kThreads / 32 : 1][4096];
     const int lane = threadIdx.x & 31;
     const long long step = (long long)gridDim.x * (kThreads / 32);
     for (long long w = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < items; w += step) {
@@ -129,14 +151,29 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const Kv4Span s, co
         const bool on0 = first + 2 * t >= 0 && first + 2 * t < it.count;
         const bool on1 = first + 2 * t + 1 >= 0 && first + 2 * t + 1 < it.count;
         uint32_t ka[8], kb[8], va[8], vb[8];
-        const T* kp = k + col + (first + g) * row_stride + 32 * t;
-        const T* vp = v + col + (first + 2 * t) * row_stride + 16 * g;
-        if (on) {
-            load16(kp, ka);
-            load16(kp + 16, kb);
+        if constexpr (sizeof(T) == 4) {
+            uint8_t* st = stage[threadIdx.x >> 5];
+            __syncwarp();                              // (the block before has been read)
+            float4 yk[kKv4BlockRows], yv[kKv4BlockRows];
+            fetch_rows(yk, k + col, row_stride, first, it.count, lane);
+            fetch_rows(yv, v + col, row_stride, first, it.count, lane);
+            stage_rows(st, yk, lane);
+            stage_rows(st + 2048, yv, lane);
+            __syncwarp();
+            load16(st, g, 4 * t, ka);
+            load16(st, g, 4 * t + 2, kb);
+            load16(st + 2048, 2 * t, 2 * g, va);
+            load16(st + 2048, 2 * t + 1, 2 * g, vb);
+        } else {
+            const T* kp = k + col + (first + g) * row_stride + 32 * t;
+            const T* vp = v + col + (first + 2 * t) * row_stride + 16 * g;
+            if (on) {
+                load16(kp, ka);
+                load16(kp + 16, kb);
+            }
+            if (on0) load16(vp, va);
+            if (on1) load16(vp + row_stride, vb);
         }
-        if (on0) load16(vp, va);
-        if (on1) load16(vp + row_stride, vb);
         if (on) {
             uint32_t c0[2], c1[2];
             const uint32_t s0 = quantise16(ka, c0, status), s1 = quantise16(kb, c1, status);
@@ -161,52 +198,66 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const Kv4Span s, co
     }
 }
 
-// Eight values from a word and its scale byte, in order.
-__device__ __forceinline__ uint4 values8(uint32_t w, uint32_t byte) {
-    const Scale2 s = scale2(byte * 0x00010001u);
-    return make_uint4(field<0>(w, s), field<1>(w, s), field<2>(w, s), field<3>(w, s));
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const uint4& x) {
-    *reinterpret_cast<uint4*>(p) = x;
-}
-__device__ __forceinline__ void store8(float* p, const uint4& x) {
-    *reinterpret_cast<float4*>(p) = make_float4(lo_f(x.x), hi_f(x.x), lo_f(x.y), hi_f(x.y));
-    *reinterpret_cast<float4*>(p + 4) = make_float4(lo_f(x.z), hi_f(x.z), lo_f(x.w), hi_f(x.w));
-}
+// The read kernel's lanes: kDims consecutive dims a lane, so that a warp's
+// store is 512 consecutive bytes of one or two rows (bf16: a whole word of
+// eight dims, fp32: half of one).
+template <class T>
+struct Out;
+template <>
+struct Out<__nv_bfloat16> {
+    static constexpr int kDims = 8;
+    static __device__ __forceinline__ void store(__nv_bfloat16* p, uint32_t w, int, const Scale2& s) {
+        __stcs(reinterpret_cast<uint4*>(p), make_uint4(field<0>(w, s), field<1>(w, s), field<2>(w, s), field<3>(w, s)));
+    }
+};
+template <>
+struct Out<float> {
+    static constexpr int kDims = 4;
+    static __device__ __forceinline__ void store(float* p, uint32_t w, int part, const Scale2& s) {
+        w >>= 8 * part;
+        const uint32_t a = field<0>(w, s), b = field<1>(w, s);
+        __stcs(reinterpret_cast<float4*>(p), make_float4(lo_f(a), hi_f(a), lo_f(b), hi_f(b)));
+    }
+};
 
 template <class T>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const Kv4Span s, T* __restrict__ k,
                                                             T* __restrict__ v, long long row_stride,
                                                             long long batch_stride, int blocks,
                                                             long long items, int* status) {
+    constexpr int kDims = Out<T>::kDims, kLanes = 128 / kDims, kRows = 32 / kLanes;   // lanes of a row, rows of a pass
     const int lane = threadIdx.x & 31;
-    const int word = lane & 15;                        // dims [8 word, 8 word + 8) of rows lane/16 + 2i
+    const int dim = lane % kLanes * kDims, word = dim / 8, part = dim % 8 / 4;
     const long long step = (long long)gridDim.x * (kThreads / 32);
     for (long long w = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < items; w += step) {
         Item it;
         if (!item_of(s, w, blocks, lane, status, it)) continue;
-        const long long col = it.b * batch_stride + it.h * 128 + 8 * word;
         const int first = it.pos0 - it.start;
+        const long long at0 = it.b * batch_stride + it.h * 128 + dim;
+        // every load first: a page that is not in the pool reads as codes of 0
+        uint32_t c[2][8 / kRows], e[2][8 / kRows];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 2 * i + (lane >> 4);
-            if (first + r < 0 || first + r >= it.count) continue;
-            const long long at = col + (first + r) * row_stride;
+        for (int i = 0; i < 8 / kRows; ++i) {
+            const int r = kRows * i + lane / kLanes;
+            c[0][i] = c[1][i] = 0x88888888u;
+            e[0][i] = e[1][i] = 0u;
+            if (!it.blk || first + r < 0 || first + r >= it.count) continue;
             if (k) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (it.blk)
-                    x = values8(*reinterpret_cast<const uint32_t*>(it.blk + r * 64 + word * 4),
-                                it.blk[kKv4KScale + r * 8 + (word >> 1)]);
-                store8(k + at, x);
+                c[0][i] = *reinterpret_cast<const uint32_t*>(it.blk + r * 64 + word * 4);
+                e[0][i] = it.blk[kKv4KScale + r * 8 + (word >> 1)];
             }
             if (v) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (it.blk)
-                    x = values8(*reinterpret_cast<const uint32_t*>(it.blk + kKv4VCode + (word >> 1) * 64 + r * 8 +
-                                                                   (word & 1) * 4),
-                                it.blk[kKv4VScale + (word >> 1) * 8 + r]);
-                store8(v + at, x);
+                c[1][i] = *reinterpret_cast<const uint32_t*>(it.blk + kKv4VCode + (word >> 1) * 64 + r * 8 + (word & 1) * 4);
+                e[1][i] = it.blk[kKv4VScale + (word >> 1) * 8 + r];
             }
+        }
+#pragma unroll
+        for (int i = 0; i < 8 / kRows; ++i) {
+            const int r = kRows * i + lane / kLanes;
+            if (first + r < 0 || first + r >= it.count) continue;
+            const long long at = at0 + (first + r) * row_stride;
+            if (k) Out<T>::store(k + at, c[0][i], part, scale2(e[0][i] * 0x00010001u));
+            if (v) Out<T>::store(v + at, c[1][i], part, scale2(e[1][i] * 0x00010001u));
         }
     }
 }
