@@ -376,11 +376,43 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
 }
 
 // ------------------------------------------------------------- joining splits
-// kJoin warps per (sequence, K/V head, row), four dims a lane; a warp adds
-// every kJoin-th split.  The lanes hold the splits' weights, so the partials'
-// loads wait for nothing but them.  Launched while the splits still run
-// (programmatic stream serialization), so that its own launch costs no time
-// after them.
+// One row of kJoin warps' work, four dims a lane: the sum over its partials,
+// rows at(0) .. at(splits - 1) of the workspace; a warp adds every kJoin-th.
+// The lanes hold the partials' weights, so their loads wait for nothing but
+// them.
+template <class At>
+__device__ __forceinline__ float add_partials(const Kv4Params& P, int splits, int first, int step, int lane, At&& at,
+                                              float4& acc) {
+    const float2* ml = reinterpret_cast<const float2*>(P.ws_ml);
+    const float4* o = reinterpret_cast<const float4*>(P.ws_o) + lane;
+    float top = -INFINITY, sum = 0.f;
+    for (int c = lane; c < splits; c += 32) top = fmaxf(top, ml[at(c)].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    for (int c0 = 0; c0 < splits; c0 += 32) {
+        float f = 0.f;                                // stays 0 for a split without keys of this row
+        if (c0 + lane < splits) {
+            const float2 y = ml[at(c0 + lane)];
+            if (y.y != 0.f) f = ex2(y.x - top);
+            sum += f * y.y;
+        }
+        const int n = min(32, splits - c0);
+#pragma unroll 4
+        for (int c = first; c < n; c += step) {
+            const float g = __shfl_sync(0xffffffffu, f, c);
+            if (g != 0.f) {
+                const float4 y = o[at(c0 + c) * (kKv4Head / 4)];
+                acc.x += g * y.x; acc.y += g * y.y; acc.z += g * y.z; acc.w += g * y.w;
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    return sum;
+}
+
+// Both joins are launched while the splits still run (programmatic stream
+// serialization), so that their own launch costs no time after them.
 template <int kJoin>
 __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
     __shared__ float4 part[8][32];
@@ -389,7 +421,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
     const uint32_t w = blockIdx.x * (8 / kJoin) + warp / kJoin, max_rows = (uint32_t)P.max_rows;
     cudaGridDependencySynchronize();                  // the partials are complete and visible
     int start, count, r = 0, h = 0, b = 0;
-    bool on = w < (uint32_t)(s.batch * s.kv_heads) * max_rows;   // below 2^31: launch_attn_kv4
+    bool on = w < (uint32_t)(s.batch * s.kv_heads) * max_rows;   // (below 2^31: launch_attn_kv4)
     if (on) {
         r = (int)(w % max_rows);
         h = (int)(w / max_rows % (uint32_t)s.kv_heads);
@@ -398,33 +430,8 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
     }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
-    if (on) {
-        const float2* ml = reinterpret_cast<const float2*>(P.ws_ml) + (long long)w * P.splits;
-        const float4* o = reinterpret_cast<const float4*>(P.ws_o + (long long)w * P.splits * kKv4Head) + lane;
-        float top = -INFINITY;
-        for (int c = lane; c < P.splits; c += 32) top = fmaxf(top, ml[c].x);
-#pragma unroll
-        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        for (int c0 = 0; c0 < P.splits; c0 += 32) {
-            float f = 0.f;                            // stays 0 for a split without keys of this row
-            if (c0 + lane < P.splits) {
-                const float2 y = ml[c0 + lane];
-                if (y.y != 0.f) f = ex2(y.x - top);
-                sum += f * y.y;
-            }
-            const int n = min(32, P.splits - c0);
-#pragma unroll 4
-            for (int c = sub; c < n; c += kJoin) {
-                const float g = __shfl_sync(0xffffffffu, f, c);
-                if (g != 0.f) {
-                    const float4 y = o[(long long)(c0 + c) * (kKv4Head / 4)];
-                    acc.x += g * y.x; acc.y += g * y.y; acc.z += g * y.z; acc.w += g * y.w;
-                }
-            }
-        }
-#pragma unroll
-        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    }
+    if (on)
+        sum = add_partials(P, P.splits, sub, kJoin, lane, [&](int c) { return (long long)w * P.splits + c; }, acc);
     if (kJoin > 1) {
         part[warp][lane] = acc;
         __syncthreads();
@@ -436,6 +443,26 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
         }
     }
     if (on) store_out(P, b, h, r, 4 * lane, acc, sum);
+}
+
+// The units of the kernel for many rows that lie in several CTAs' chunks
+// (Kv4Unit): kUnitCtas CTAs a unit, a warp a row at a time.
+constexpr int kUnitCtas = 16;
+__global__ void __launch_bounds__(256) attn_kv4_join_units_kernel(const Kv4Params P) {
+    const int unit = (int)(blockIdx.x / kUnitCtas), lane = threadIdx.x & 31;
+    const Kv4Unit u = unit_of(P, unit / P.span.kv_heads);
+    cudaGridDependencySynchronize();
+    if (u.pages == 0) return;
+    const int chunk = P.ws_unit[0], page = P.ws_unit[1 + unit], c0 = page / chunk;
+    const int splits = (page + u.pages - 1) / chunk - c0 + 1;
+    if (splits == 1) return;                          // its rows are finished
+    const int rows = min(u.rows - u.r0, 256);
+    for (int row = (int)(blockIdx.x % kUnitCtas) * 8 + ((int)threadIdx.x >> 5); row < rows; row += kUnitCtas * 8) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float sum = add_partials(
+            P, splits, 0, 1, lane, [&](int c) { return unit_slot(c0 + c, c == 0) * 256 + row; }, acc);
+        store_out(P, u.b, unit % P.span.kv_heads, u.r0 + row, 4 * lane, acc, sum);
+    }
 }
 
 template <int NB>
@@ -504,22 +531,6 @@ int sm_count() {
     return n > 0 ? n : 148;
 }
 
-// Splits of the pages of a 256-row tile: minimise rounds of one CTA an SM x
-// (pages of a split + a fixed cost of about 4 pages: prologue, epilogue, join).
-int tile_splits(long long units, int pages, int sms) {
-    int best = 1;
-    long long best_cost = -1;
-    for (int c = 1; c <= 64 && c <= (pages + 1) / 2; ++c) {
-        const long long rounds = (units * c + sms - 1) / sms;
-        const long long cost = rounds * ((pages + c - 1) / c + (c > 1 ? 4 : 2));
-        if (best_cost < 0 || cost < best_cost) {
-            best_cost = cost;
-            best = c;
-        }
-    }
-    return best;
-}
-
 }  // namespace
 
 int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStream_t stream) {
@@ -545,14 +556,23 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     const int nb = P.max_rows > 8 ? 2 : 1, tile_rows = tiles ? 256 : 8 * nb;
     P.row_tiles = (P.max_rows + tile_rows - 1) / tile_rows;
     const long long units = (long long)s.batch * s.kv_heads * P.row_tiles;
+    long long grid = units, slots = 0;   // slots: rows of the workspace
     // Keys of a row tile, at most (starts on the device: the capacity's).
     long long keys = s.starts ? cap : (long long)s.start + s.rows;
-    if (a.window) {
-        const long long span = (long long)(tile_rows / P.group + 2 + (long long)a.tokens) + P.window_rows + P.sink_rows;
-        keys = std::min(keys, span);
-    }
+    if (a.window)
+        keys = std::min(keys, tile_rows / P.group + 2 + (long long)a.tokens + P.window_rows + P.sink_rows);
     if (tiles) {
-        P.splits = tile_splits(units, (int)((keys + kKv4PageRows - 1) / kKv4PageRows), sm_count());
+        // A CTA an SM takes one unit after the other.  Units that do not divide
+        // evenly over the SMs are cut: the CTAs share all units' pages, which
+        // costs a piece more for each (about three pages) and the join (three).
+        P.splits = 1;
+        const long long sms = sm_count(), pages = (keys + kKv4PageRows - 1) / kKv4PageRows;
+        P.chunked = (units + sms - 1) / sms * (pages + 3) > units * (pages + 3) / sms + 6 && units < 8 * sms &&
+                    (long long)s.batch * P.row_tiles <= kKv4ChunkPairs && units * s.map_stride < 0x7fffffffLL;
+        if (P.chunked) {
+            grid = sm_count();
+            slots = 2 * 256 * grid;
+        }
     } else {
         const int* at_once = nullptr;
         const int rf = nb == 1 ? rows_fit<1>(&at_once) : rows_fit<2>(&at_once);
@@ -576,41 +596,44 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
             if ((1 << i) <= want && units <= at_once[i]) c = 1 << i;
         P.cluster = c > 0 && a_warp(c) <= a_warp(want) + 2;
         P.splits = P.cluster ? c : (int)want;
+        grid = units * P.splits;
+        // (units * want is at most what the device runs at once)
+        if (P.splits > 1 && !P.cluster) slots = (long long)s.batch * s.kv_heads * P.max_rows * P.splits;
     }
-    if ((long long)s.batch * s.kv_heads * P.max_rows > 0x7fffffffLL) P.splits = 1;   // the join counts rows in 31 bits
-    const long long grid = units * P.splits;
     if (grid > 0x7fffffffLL) {
         set_error("attn_kv4: too many rows for one launch");
         return KVP_ERR_ARG;
     }
-    const long long slots = (long long)s.batch * s.kv_heads * P.max_rows * P.splits;
     void* ws = nullptr;
-    if (P.splits > 1 && !P.cluster) {
+    if (slots > 0) {
+        const size_t rows_bytes = (size_t)slots * (kKv4Head + 2) * sizeof(float);
         cudaMemPool_t pool = nullptr;
         KVP_CUDA(workspace_pool(&pool));
-        KVP_CUDA(cudaMallocFromPoolAsync(&ws, (size_t)slots * (kKv4Head + 2) * sizeof(float), pool, stream));
+        KVP_CUDA(cudaMallocFromPoolAsync(&ws, rows_bytes + (P.chunked ? (size_t)(1 + units) * sizeof(int) : 0), pool, stream));
         P.ws_o = static_cast<float*>(ws);
         P.ws_ml = P.ws_o + slots * kKv4Head;
+        P.ws_unit = reinterpret_cast<int*>(P.ws_ml + slots * 2);
     }
     int launched = tiles   ? launch_kv4_tiles(P, (unsigned)grid, stream)
                    : nb == 1 ? launch_rows<1>(P, (unsigned)grid, stream)
                              : launch_rows<2>(P, (unsigned)grid, stream);
     if (ws) {
         if (launched == KVP_OK) {
-            const long long rows = slots / P.splits;
             cudaLaunchAttribute early;
             early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
             early.val.programmaticStreamSerializationAllowed = 1;
             cudaLaunchConfig_t cfg = {};
-            // a few splits: one warp a row; many: eight share them
-            const bool many = P.splits > 8;
-            cfg.gridDim = dim3((unsigned)(many ? rows : (rows + 7) / 8));
             cfg.blockDim = dim3(256);
             cfg.stream = stream;
             cfg.attrs = &early;
             cfg.numAttrs = 1;
-            const cudaError_t e = many ? cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel<8>, P)
-                                       : cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel<1>, P);
+            // a few splits: one warp a row; many: eight share them
+            const long long rows = slots / P.splits;
+            const bool many = P.splits > 8;
+            cfg.gridDim = dim3((unsigned)(tiles ? units * kUnitCtas : many ? rows : (rows + 7) / 8));
+            const cudaError_t e = tiles  ? cudaLaunchKernelEx(&cfg, attn_kv4_join_units_kernel, P)
+                                  : many ? cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel<8>, P)
+                                         : cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel<1>, P);
             if (e != cudaSuccess) launched = cuda_status(e, "attn_kv4 join");
         }
         const cudaError_t e = cudaFreeAsync(ws, stream);

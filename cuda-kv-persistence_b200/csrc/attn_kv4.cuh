@@ -14,11 +14,13 @@ struct Kv4Params {
     int* status;
     float* ws_o;             // partial O of split c: [sequence][K/V head][row][split][128]
     float* ws_ml;            // its max (log2 units) and sum: [...][split][2]
+    int* ws_unit;            // chunked: [0] pages of a CTA, [1 + unit] the unit's first page in the list of all
     long long window_rows;   // window * tokens (0: all keys)
     int sink_rows;           // sinks * tokens, at most the capacity
     int group, max_rows;     // query heads per K/V head; rows * group
     int tokens, row_tiles, splits;
     int cluster;             // the splits of a row tile are one cluster and join by themselves
+    int chunked;             // (many rows) the CTAs share the list of all units' pages evenly: see Kv4Unit
     float scale_log2;        // log2(e) / sqrt(128)
     float rise;              // kRise in score units
 };
@@ -46,6 +48,38 @@ __device__ __forceinline__ __nv_bfloat16* out_row(const Kv4Params& P, int b, int
     return static_cast<__nv_bfloat16*>(P.attn.out) + b * P.attn.out_batch_stride +
            (long long)(r / P.group) * P.attn.out_row_stride + (long long)(h * P.group + r % P.group) * kKv4Head;
 }
+
+// The units of the kernel for many rows: 256 query rows of one sequence and
+// K/V head, against the pages that any of them sees (those of the sinks
+// below the window, then the window's).  Unit u = pair * kv_heads + head,
+// pairs of (row tile, sequence) with the last rows, the longest spans, first.
+// Chunked, CTA i takes pages [i C, (i + 1) C) of the list of all units' pages;
+// a piece that is not its whole unit is a partial, in slot 2 i + 1 if it
+// begins the unit (it is the CTA's last then), 2 i if not (its first).
+struct Kv4Unit {
+    int b, start, end, rows, r0;       // rows = count * group; this unit's [r0, r0 + 256)
+    int na, b0, pages;                 // pages [0, na) and [b0, b0 + pages - na); 0: nothing to do
+    Sees first, last;                  // what its first and last row see
+    bool refused;                      // the sequence's start or count does not fit
+};
+__device__ __forceinline__ Kv4Unit unit_of(const Kv4Params& P, int pair) {
+    Kv4Unit u;
+    u.b = pair % P.span.batch;
+    u.r0 = (P.row_tiles - 1 - pair / P.span.batch) * 256;
+    u.pages = 0;
+    int count;
+    u.refused = !sequence(P.span, u.b, u.start, count);
+    u.rows = u.refused ? 0 : count * P.group;
+    if (u.r0 >= u.rows) return u;
+    u.end = u.start + count;
+    u.first = sees(P, u.start + u.r0 / P.group, u.end);
+    u.last = sees(P, u.start + (min(u.r0 + 256, u.rows) - 1) / P.group, u.end);
+    u.b0 = u.first.lo / kKv4PageRows;
+    u.na = min((min(P.sink_rows, u.last.hi) + kKv4PageRows - 1) / kKv4PageRows, u.b0);
+    u.pages = u.na + (u.last.hi + kKv4PageRows - 1) / kKv4PageRows - u.b0;
+    return u;
+}
+__device__ __forceinline__ long long unit_slot(int cta, bool begins) { return 2LL * cta + (begins ? 1 : 0); }
 
 // A row's partial O and (max, sum) of one split.
 __device__ __forceinline__ long long ws_slot(const Kv4Params& P, int b, int h, int r, int split) {
@@ -80,6 +114,8 @@ __device__ __forceinline__ void put(const Kv4Params& P, int b, int h, int r, int
 }
 
 }  // namespace kv4_dev
+
+constexpr int kKv4ChunkPairs = 1152;     // (row tile, sequence) pairs that the CTAs of a chunked launch add up
 
 // The kernel for many query rows (attn_kv4_sm100.cu): P.row_tiles of 256 rows.
 int launch_kv4_tiles(const Kv4Params& P, unsigned grid, cudaStream_t stream);

@@ -4,7 +4,8 @@
 // Bound by the two products: 4 * 128 flops a (query row, key), against 144
 // bytes a key that every 256 query rows read again from L2.  CTA = two
 // 128-row query tiles of one K/V head (rows r = i * group + g, so grouped
-// heads fill a tile) x a range of 128-key pages.  Warp roles (384 threads):
+// heads fill a tile) x a range of 128-key pages, one such unit after the
+// other (Kv4Unit).  Warp roles (384 threads):
 //   warps 0, 2, 3   expand the cache: units of 32 rows of K or V in turn,
 //                   16-byte words from global memory (one unit ahead), fields
 //                   to bf16 in registers, 16-byte stores into the 128B-
@@ -57,12 +58,69 @@ struct __align__(1024) Smem {
     uint64_t bar_mma_done;      // every issued MMA landed (TMEM may be freed)
     uint32_t tmem_base;
     int abort_flag;
-    // the CTA's item, for what the softmax seldom needs (not held in registers)
-    volatile int batch, head, rows, row0, split, u0, na, b0, any_bad, releaser, free0, free1;
+    int scan[kThreads / 32];
+    // The CTA's work list: what it does next (thread 0 moves it on).
+    volatile int pair, head, off, left, pos;
+    volatile int any_bad[2];    // a page of the piece is not in the pool; the other for the next piece
+    // The piece, for what the softmax seldom needs (not held in registers)
+    volatile int batch, rows, row0, u0, n_tiles, rot, na, b0, partial, releaser, free_n;
 };
 
 // Bits [0, n) set.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// 128 columns of an S row of which vis says which are visible (32 a word; a
+// warp's rows agree on most words) -> P, their sum; and their max.  A hidden
+// key's weight is 0: everything on MUFU, whose 2^-inf is 0.
+__device__ __forceinline__ void load_visible(uint32_t s_addr, uint32_t vis, uint32_t (&y)[32]) {
+    KVP_TMEM_LD32(s_addr, y);
+    KVP_TMEM_WAIT_LD_DEP(y);
+    if (__any_sync(0xffffffffu, vis != 0xffffffffu)) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+            if (!(vis >> c & 1u)) y[c] = 0xFF800000u;   // -inf
+    }
+}
+__device__ __forceinline__ float exp_visible(uint32_t s_addr, float m, float sl2, const uint32_t (&vis)[4],
+                                             uint32_t (&pk)[64]) {
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+        if (__all_sync(0xffffffffu, vis[h] == 0u)) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) pk[16 * h + c] = 0u;
+            continue;
+        }
+        uint32_t y[32];
+        load_visible(s_addr + 32 * h, vis[h], y);
+        float part[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(y[c]), sl2, -m));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(y[c + 1]), sl2, -m));
+            part[0] += p0;
+            part[1] += p1;
+            pk[16 * h + (c >> 1)] = pack_bf16(p0, p1);
+        }
+        sum += part[0] + part[1];
+    }
+    return sum;
+}
+__device__ __forceinline__ float max_visible(uint32_t s_addr, const uint32_t (&vis)[4]) {
+    float m = -INFINITY;
+#pragma unroll 1
+    for (int h = 0; h < 4; ++h) {
+        const uint32_t v = h == 0 ? vis[0] : h == 1 ? vis[1] : h == 2 ? vis[2] : vis[3];
+        if (__all_sync(0xffffffffu, v == 0u)) continue;
+        uint32_t y[32];
+        load_visible(s_addr + 32 * h, v, y);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(y[c]));
+        m = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+    }
+    return m;
+}
 
 // The four words and scale bytes of a lane's 16 bytes as four bf16 chunks.
 __device__ __forceinline__ void expand4(uint8_t* tile, const uint32_t (&off)[4], uint32_t w0, uint32_t w1,
@@ -71,6 +129,109 @@ __device__ __forceinline__ void expand4(uint8_t* tile, const uint32_t (&off)[4],
     *reinterpret_cast<uint4*>(tile + off[1]) = make_uint4(field<0>(w1, s01), field<1>(w1, s01), field<2>(w1, s01), field<3>(w1, s01));
     *reinterpret_cast<uint4*>(tile + off[2]) = make_uint4(field<0>(w2, s23), field<1>(w2, s23), field<2>(w2, s23), field<3>(w2, s23));
     *reinterpret_cast<uint4*>(tile + off[3]) = make_uint4(field<0>(w3, s23), field<1>(w3, s23), field<2>(w3, s23), field<3>(w3, s23));
+}
+
+constexpr int kMinPages = 4;                  // of a CTA's share: a piece costs about three pages more
+
+__device__ __forceinline__ void init_barriers(Smem& sm) {
+    for (int q = 0; q < 2; ++q) {
+        mbar_init(&sm.bar_q[q], 128);
+        mbar_init(&sm.bar_s_full[q], 1);
+        mbar_init(&sm.bar_p_full[q], 128);
+        mbar_init(&sm.bar_o_done[q], 1);
+    }
+    for (int i = 0; i < kKStages; ++i) {
+        mbar_init(&sm.bar_kfull[i], kUnits / 2);
+        mbar_init(&sm.bar_kempty[i], 1);
+    }
+    for (int i = 0; i < kVStages; ++i) {
+        mbar_init(&sm.bar_vfull[i], kUnits / 2);
+        mbar_init(&sm.bar_vempty[i], 1);
+    }
+    mbar_init(&sm.bar_mma_done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
+}
+
+// A CTA's piece of a unit: its pages [u0, u0 + n_tiles).
+// Its tiles go round from the first that every row sees whole: that gives each
+// row its max, and the tiles with hidden keys need one pass like the others.
+struct Piece {
+    Kv4Unit u;
+    int u0, n_tiles, rot;
+    bool two;                                 // the second query tile has rows
+    __device__ __forceinline__ Piece(const Kv4Params& P, Smem& sm) {
+        u = unit_of(P, sm.pair);
+        u0 = sm.off;
+        n_tiles = min(u.pages - u0, sm.left);
+        two = u.r0 + 128 < u.rows;
+        rot = free0() < free1() ? free0() : 0;
+    }
+    // tiles [free0, free1) in the order of their pages: every row sees them whole
+    __device__ __forceinline__ int free0() const {
+        return max(u.na + (u.last.lo + kBN - 1) / kBN - u.b0 - u0, 0);
+    }
+    __device__ __forceinline__ int free1() const { return min(u.na + u.first.hi / kBN - u.b0 - u0, n_tiles); }
+    __device__ __forceinline__ int page_pos(int j) const {   // position page of tile j
+        j += rot;
+        const int i = u0 + (j < n_tiles ? j : j - n_tiles);
+        return i < u.na ? i : i - u.na + u.b0;
+    }
+    // Every thread: the piece's pages are looked up once, the roles may start after it.
+    __device__ __forceinline__ void set_up(const Kv4Params& P, Smem& sm, int turn) const {
+        for (int j = threadIdx.x; j < n_tiles; j += kThreads)
+            if (page_of(P.span, u.b, page_pos(j)) < 0) sm.any_bad[turn & 1] = 1;
+        if (threadIdx.x == 0) {
+            sm.any_bad[(turn + 1) & 1] = 0;
+            sm.batch = u.b;
+            sm.rows = u.rows;
+            sm.row0 = u.r0;
+            sm.u0 = u0;
+            sm.n_tiles = n_tiles;
+            sm.rot = rot;
+            sm.na = u.na;
+            sm.b0 = u.b0;
+            sm.partial = n_tiles < u.pages;
+            sm.releaser = two ? 256 : 128;
+            sm.free_n = max(free1() - free0(), 0);
+            if (P.chunked && u0 == 0) P.ws_unit[1 + sm.pair * P.span.kv_heads + sm.head] = sm.pos;
+        }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (sm.any_bad[turn & 1] && threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_MAP);
+    }
+};
+
+// Every thread: the piece is done; thread 0 moves the list on.
+__device__ __forceinline__ void done(const Kv4Params& P, Smem& sm, const Piece& w) {
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int pair = sm.pair, head = sm.head + 1;
+        const int left = sm.left - w.n_tiles;
+        if (left > 0 && head == P.span.kv_heads) {
+            head = 0;
+            do ++pair;
+            while (unit_of(P, pair).pages == 0);        // left > 0: there is one
+        }
+        sm.pair = pair;
+        sm.head = head;
+        sm.off = 0;
+        sm.pos = sm.pos + w.n_tiles;
+        sm.left = left;
+        if (left > 0) {
+            uint64_t* bars[] = {sm.bar_q, sm.bar_s_full, sm.bar_p_full, sm.bar_o_done, sm.bar_kfull, sm.bar_kempty,
+                                sm.bar_vfull, sm.bar_vempty, &sm.bar_mma_done};
+            const int n[] = {2, 2, 2, 2, kKStages, kKStages, kVStages, kVStages, 1};
+            for (int i = 0; i < 9; ++i)
+                for (int e = 0; e < n[i]; ++e)
+                    asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bars[i] + e)) : "memory");
+            init_barriers(sm);
+        }
+    }
+    __syncthreads();
+    tc_fence_after();
 }
 
 __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __grid_constant__ Kv4Params P) {
@@ -83,108 +244,109 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const Kv4Span& s = P.span;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // CTA = (split, query tile pair, K/V head, sequence), split fastest, last rows
-    // (the longest spans) first
-    uint32_t x = blockIdx.x;
-    const int split = (int)(x % (uint32_t)P.splits);
-    x /= (uint32_t)P.splits;
-    const int h = (int)(x % (uint32_t)s.kv_heads);
-    x /= (uint32_t)s.kv_heads;
-    const int b = (int)(x % (uint32_t)s.batch);
-    const int r0 = (P.row_tiles - 1 - (int)(x / (uint32_t)s.batch)) * 256;
-    int start, count;
-    if (!sequence(s, b, start, count)) {
-        if (threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_MAP);
-        return;
-    }
-    const int rows = count * P.group;
-    if (r0 >= rows) return;
-    const int end = start + count;
-    const Sees first = sees(P, start + r0 / P.group, end);
-    const Sees last = sees(P, start + (min(r0 + 256, rows) - 1) / P.group, end);
-    // pages: those of the sinks below the window, then the window's
-    const int b0 = first.lo / kBN, na = min((min(P.sink_rows, last.hi) + kBN - 1) / kBN, b0);
-    const int total = na + (last.hi + kBN - 1) / kBN - b0, per = (total + P.splits - 1) / P.splits;
-    const int u0 = min(split * per, total), n_tiles = min(u0 + per, total) - u0;
-    const bool two = r0 + 128 < rows;             // the second query tile has rows
-    auto page_pos = [&](int j) {                  // position page of the CTA's tile j
-        const int u = u0 + j;
-        return u < na ? u : u - na + b0;
-    };
-    auto lookup = [&](int j) { return j < n_tiles ? page_of(s, b, page_pos(j)) : 0; };
-
-                    const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
-                    const uint8_t* head = static_cast<const uint8_t*>(s.pages) + h * kKv4PageHeadBytes;
-                    const int units = n_tiles * kUnits;
-                    uint4 c[4];
-                    uint32_t sc[4];
-                    auto load = [&](int n, int page) {
-                        const int part = (n >> 2) & 1;
-                        const uint8_t* p = head + (unsigned long long)(uint32_t)max(page, 0) * page_bytes +
-                                           (n & 3) * 4 * kKv4BlockBytes;
-                        const uint8_t* pc = p + (part ? kKv4VCode : 0) + lane * 16;
-                        const uint8_t* ps = p + (part ? kKv4VScale : kKv4KScale) + lane * 2;
+    // Where this CTA's work begins, and how many pages it takes.
+    int pair = 0, head = 0, off = 0, left = 0, pos = 0;
+    if (P.chunked) {
+        // prefix sums of the pairs' pages, three pairs a thread
+        const int pairs = P.row_tiles * s.batch;
+        int n[3], mine = 0;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            c[i] = *reinterpret_cast<const uint4*>(pc + i * kKv4BlockBytes);
-                            sc[i] = *reinterpret_cast<const uint16_t*>(ps + i * kKv4BlockBytes);
-                        }
-                    };
-                    // an expander's unit; its first is on its way while the CTA sets up
-    int n = warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : units;
-                    int page = lookup(n / kUnits), page1 = lookup((n + kExpanders) / kUnits);
-                    if (n < units) load(n, page);
-
+        for (int i = 0; i < 3; ++i) {
+            const int p = 3 * (int)threadIdx.x + i;
+            n[i] = p < pairs ? unit_of(P, p).pages : 0;
+            mine += n[i];
+        }
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 31) sm.scan[warp] = upto;
+        __syncthreads();
+        int before = upto - mine, all = 0;
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) before += sm.scan[w];
+            all += sm.scan[w];
+        }
+        all *= s.kv_heads;
+        const int chunk = max((all + (int)gridDim.x - 1) / (int)gridDim.x, kMinPages);
+        pos = (int)min((long long)blockIdx.x * chunk, (long long)all);
+        left = min(chunk, all - pos);
+        if (blockIdx.x == 0 && threadIdx.x == 0) P.ws_unit[0] = chunk;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const int r = pos - before * s.kv_heads;   // pages into this pair's kv_heads units
+            if (left > 0 && r >= 0 && r < n[i] * s.kv_heads) {
+                sm.pair = 3 * (int)threadIdx.x + i;
+                sm.head = r / n[i];
+                sm.off = r % n[i];
+            }
+            before += n[i];
+        }
+    } else {
+        pair = (int)(blockIdx.x / (uint32_t)s.kv_heads);
+        head = (int)(blockIdx.x % (uint32_t)s.kv_heads);
+        left = unit_of(P, pair).pages;
+        if (threadIdx.x == 0) {
+            sm.pair = pair;
+            sm.head = head;
+            sm.off = off;
+        }
+    }
+    // the refused sequences are reported once
+    if (threadIdx.x == 0)
+        for (int i = (int)blockIdx.x; i < s.batch; i += (int)gridDim.x)
+            if (unit_of(P, i).refused) atomicOr(P.status, KVP_STATUS_MAP);
+    if (left == 0) return;
     if (threadIdx.x == 0) {
-        for (int q = 0; q < 2; ++q) {
-            mbar_init(&sm.bar_q[q], 128);
-            mbar_init(&sm.bar_s_full[q], 1);
-            mbar_init(&sm.bar_p_full[q], 128);
-            mbar_init(&sm.bar_o_done[q], 1);
-        }
-        for (int i = 0; i < kKStages; ++i) {
-            mbar_init(&sm.bar_kfull[i], kUnits / 2);
-            mbar_init(&sm.bar_kempty[i], 1);
-        }
-        for (int i = 0; i < kVStages; ++i) {
-            mbar_init(&sm.bar_vfull[i], kUnits / 2);
-            mbar_init(&sm.bar_vempty[i], 1);
-        }
-        mbar_init(&sm.bar_mma_done, 1);
+        sm.left = left;
+        sm.pos = pos;
         sm.abort_flag = 0;
-        sm.batch = b;
-        sm.head = h;
-        sm.rows = rows;
-        sm.row0 = r0;
-        sm.split = split;
-        sm.u0 = u0;
-        sm.na = na;
-        sm.b0 = b0;
-        sm.any_bad = 0;
-        // the CTA's tiles that every row sees whole
-        sm.free0 = na + (last.lo + kBN - 1) / kBN - b0 - u0;
-        sm.free1 = na + first.hi / kBN - b0 - u0;
-        sm.releaser = two ? 256 : 128;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        fence_proxy_async_smem();
+        sm.any_bad[0] = sm.any_bad[1] = 0;
+        init_barriers(sm);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(&sm.tmem_base)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    bool bad = false;
-    for (int j = threadIdx.x; j < n_tiles; j += kThreads) bad |= lookup(j) < 0;
     tc_fence_before();
-    const bool any_bad = __syncthreads_or(bad);   // some page is not in the pool: its keys are masked
+    __syncthreads();
     tc_fence_after();
-    if (any_bad) {                                // (every thread writes the same, its own reads follow)
-        sm.any_bad = 1;
-        sm.free1 = 0;
-    }
     const uint32_t tmem = sm.tmem_base;
+
+    // Both sides of the role split go through the same pieces, with the same
+    // three barriers for each.
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+        for (int turn = 0; sm.left > 0; ++turn) {
+            const Piece w(P, sm);
+            const int n_tiles = w.n_tiles, h = sm.head;
+            const bool two = w.two;
+            auto lookup = [&](int j) { return j < n_tiles ? page_of(s, w.u.b, w.page_pos(j)) : 0; };
+            const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
+            const uint8_t* pool = static_cast<const uint8_t*>(s.pages) + h * kKv4PageHeadBytes;
+            const int units = n_tiles * kUnits;
+            uint4 c[4];
+            uint32_t sc[4];
+            auto load = [&](int n, int page) {
+                const int part = (n >> 2) & 1;
+                const uint8_t* p = pool + (unsigned long long)(uint32_t)max(page, 0) * page_bytes +
+                                   (n & 3) * 4 * kKv4BlockBytes;
+                const uint8_t* pc = p + (part ? kKv4VCode : 0) + lane * 16;
+                const uint8_t* ps = p + (part ? kKv4VScale : kKv4KScale) + lane * 2;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    c[i] = *reinterpret_cast<const uint4*>(pc + i * kKv4BlockBytes);
+                    sc[i] = *reinterpret_cast<const uint16_t*>(ps + i * kKv4BlockBytes);
+                }
+            };
+            // an expander's unit of 32 rows; its first is on its way while the CTA sets up
+            int n = warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : units;
+            int page = lookup(n / kUnits), page1 = lookup((n + kExpanders) / kUnits);
+            if (n < units) load(n, page);
+            w.set_up(P, sm, turn);
         if (warp != 1) {
             // ============================ expanders ===========================
             const int g = lane >> 2, t = lane & 3;
@@ -236,7 +398,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 if (lane == 0) mbar_arrive(part ? &sm.bar_vfull[st] : &sm.bar_kfull[st]);
             }
         } else {
-            if (any_bad && lane == 0) atomicOr(P.status, KVP_STATUS_MAP);
             // ============================ MMA issuer ==========================
             if (lane == 0) {
                 constexpr uint32_t idS = idesc_bf16(false);
@@ -308,12 +469,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             }
             __syncwarp();
         }
+            done(P, sm, w);
+        }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+        for (int turn = 0; sm.left > 0; ++turn) {
         // ========================== softmax + epilogue ========================
         const int qt = (warp - 4) >> 2;
         const int row = (warp & 3) * 32 + lane;        // query row in tile == TMEM lane
-        const bool active = qt == 0 || two;            // this query tile has rows
+        const Piece w(P, sm);
+        w.set_up(P, sm, turn);
+        const bool any_bad = sm.any_bad[turn & 1];
+        const int h = sm.head, n_tiles = w.n_tiles, r0 = w.u.r0, rows = w.u.rows;
+        const bool active = qt == 0 || w.two;          // this query tile has rows
         // A row past the last (Q is 0, never stored) takes every key; a warp of
         // such rows does no softmax.
         Sees mine = {0, 0};
@@ -322,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             // rows past the last are zero
             const int rw = r0 + 128 * qt + (warp & 3) * 32, sub = lane >> 4, chunk = lane & 15;
             int g = (rw + sub) % P.group;              // row r = i * group + g
-            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(P.attn.q) + b * P.attn.q_batch_stride +
+            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(P.attn.q) + w.u.b * P.attn.q_batch_stride +
                                        (long long)((rw + sub) / P.group) * P.attn.q_row_stride +
                                        (h * P.group + g) * kKv4Head + 8 * chunk;
             const long long wrap = P.attn.q_row_stride - P.group * kKv4Head;
@@ -337,12 +505,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             cp_async_wait_all();
             fence_proxy_async_smem();
             mbar_arrive(&sm.bar_q[qt]);
-            if (rw + lane < rows) mine = sees(P, start + (rw + lane) / P.group, end);
+            if (rw + lane < rows) mine = sees(P, w.u.start + (rw + lane) / P.group, w.u.end);
             else if (rw < rows) mine.hi = 0x7fffffff;
         }
         const uint32_t s_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u * qt;
         const uint32_t o_tm = s_tm + 256u;
-        const float sl2 = P.scale_log2;
         float m_run = -INFINITY, l_run = 0.f;          // m in log2 units
         bool ok = true;
         const int my_tiles = active ? n_tiles : 0;
@@ -362,47 +529,50 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             }
             uint32_t pk[64];
             float rsum = 0.f, m_new = m_run;
-            bool masked = j < sm.free0 || j >= sm.free1, none = masked;
+            uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            // gone: this row sees no key here
+            bool masked = any_bad || j >= sm.free_n, gone = false, some_gone = false, all_gone = false;
             if (masked) {
                 // columns [0, sink) and [lo, hi) are visible
-                const int u = sm.u0 + j, pos = u < sm.na ? u : u - sm.na + sm.b0, key0 = pos * kBN;
+                int u = j + sm.rot;
+                u = sm.u0 + (u < sm.n_tiles ? u : u - sm.n_tiles);
+                const int pos = u < sm.na ? u : u - sm.na + sm.b0, key0 = pos * kBN;
                 int hi = mine.hi - key0;
-                if (sm.any_bad && page_of(s, sm.batch, pos) < 0) hi = 0;
+                if (any_bad && page_of(s, sm.batch, pos) < 0) hi = 0;
                 const int sink = P.sink_rows - key0, lo = mine.lo - key0;
-                masked = false;
-#pragma unroll 1
-                for (int c0 = 0; c0 < kBN; c0 += 32) {
-                    const uint32_t vis = below(hi - c0) & (~below(lo - c0) | below(sink - c0));
-                    if (__any_sync(0xffffffffu, vis != 0u)) none = false;
-                    if (__all_sync(0xffffffffu, vis == 0xffffffffu)) continue;
-                    masked = true;
-                    uint32_t y[32];
-                    KVP_TMEM_LD32(s_tm + c0, y);
-                    KVP_TMEM_WAIT_LD_DEP(y);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (!(vis >> c & 1u)) y[c] = 0xFF800000u;   // -inf
-                    KVP_TMEM_ST32(s_tm + c0, y);
-                }
-                tmem_wait_st();
+                for (int e = 0; e < 4; ++e)
+                    vis[e] = below(hi - 32 * e) & (~below(lo - 32 * e) | below(sink - 32 * e));
+                masked = __any_sync(0xffffffffu, (vis[0] & vis[1] & vis[2] & vis[3]) != (vis[0] | vis[1] | vis[2] | vis[3]) ||
+                                                     vis[0] + 1u > 1u);
+                // (a warp whose rows each see all or nothing, two frames' rows,
+                // takes the passes without masks)
+                gone = (vis[0] | vis[1] | vis[2] | vis[3]) == 0u;
+                some_gone = __any_sync(0xffffffffu, gone);
+                all_gone = __all_sync(0xffffffffu, gone);
             }
             const bool fresh = m_run == -INFINITY;     // no key seen yet
-            const bool skip = !none && __all_sync(0xffffffffu, fresh);
-            // Exponentials against the running max; a row whose sum overgrows,
-            // or that has none yet, takes the tile's max and does them again.
+            const bool skip = __any_sync(0xffffffffu, fresh && !gone);   // the max first
+            // Exponentials against the running max; rows whose sum overgrows take
+            // the tile's max and do them again.  Where a row sees its first key
+            // the max comes first.
 #pragma unroll 1
             for (int attempt = skip ? 1 : 0;; ++attempt) {
-                if (attempt != 1 || !skip) {
-                    // (a row without keys keeps max -inf: subtract 0, every P is 0)
+                if ((attempt != 1 || !skip) && !all_gone) {
+                    // (a row without keys keeps max -inf: subtract 0)
                     const float mm = m_new == -INFINITY ? 0.f : m_new;
-                    // a hidden key's weight has to be 0: all of a masked tile on MUFU
-                    rsum = masked ? exp_row<false, 4, 0u>(s_tm, mm, sl2, kBN, pk)
-                                  : exp_row<false>(s_tm, mm, sl2, kBN, pk);
+                    rsum = masked ? exp_visible(s_tm, mm, P.scale_log2, vis, pk)
+                                  : exp_row<false, 4, 0u>(s_tm, mm, P.scale_log2, kBN, pk);
                 }
-                const bool redo = skip ? attempt == 1 : attempt == 0 && !none && (fresh || !(rsum <= kRedoSum));
+                const bool redo = !gone && (skip ? attempt == 1 : attempt == 0 && !(rsum <= kRedoSum));
                 if (!__any_sync(0xffffffffu, redo)) break;
-                const float tmax = max_row<false>(s_tm, kBN);
-                if (redo) m_new = fmaxf(m_run, tmax * sl2);
+                const float tmax = masked ? max_visible(s_tm, vis) : max_row<false>(s_tm, kBN);
+                if (redo) m_new = fmaxf(m_run, tmax * P.scale_log2);
+            }
+            if (some_gone && gone) {
+                rsum = 0.f;
+#pragma unroll
+                for (int c = 0; c < 64; ++c) pk[c] = 0u;
             }
             const float alpha = m_new == m_run ? 1.f : ex2_approx(m_run - m_new);
             l_run = l_run * alpha + rsum;
@@ -430,26 +600,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
         }
         // A warp's rows go out through its own rows of the Q tile (every S
         // has landed): a row's 128 bytes by eight lanes, four rows a store.
-        const int eb = sm.batch, eh = sm.head, es = sm.split, er = sm.rows, r = sm.row0 + 128 * qt + row;
+        const int er = sm.rows, r = sm.row0 + 128 * qt + row;
+        const bool partial = sm.partial;
         if (ok && my_tiles > 0) ok = warp_wait(&sm.bar_o_done[qt], 0, sm, P.status);
         tc_fence_after();
         uint8_t* stage = sm.q[qt] + (warp & 3) * 32 * 128;
         const int rw = r - lane, sub = lane >> 3, chunk = lane & 7;
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;         // a row without keys is 0
-        if (P.splits > 1 && ok && active && r < er)                 // (a split without pages: -inf, 0)
-            *ws_ml(P, eb, eh, r, es) = make_float2(m_run, l_run);
-        // row rw + sub + 4 i of the workspace (rows splits * 512 bytes apart) or of the output
-        uint8_t* ws = P.splits > 1 ? reinterpret_cast<uint8_t*>(ws_o(P, eb, eh, rw + sub, es)) + 16 * chunk : nullptr;
-        const long long ws_step = 4LL * P.splits * kKv4Head * 4;
-        uint8_t* out = reinterpret_cast<uint8_t*>(static_cast<__nv_bfloat16*>(P.attn.out) + eb * P.attn.out_batch_stride +
-                                                  (long long)eh * P.group * kKv4Head) + 16 * chunk;
-        const int step = P.splits > 1 ? 32 : 64;                    // dims that make 128 bytes
+        // row rw + sub + 4 i of the workspace or of the output
+        const long long slot = unit_slot((int)blockIdx.x, sm.u0 == 0) * 256 + 128 * qt + (warp & 3) * 32;
+        if (partial && ok && active)
+            *reinterpret_cast<float2*>(P.ws_ml + (slot + lane) * 2) = make_float2(m_run, l_run);
+        uint8_t* ws = reinterpret_cast<uint8_t*>(P.ws_o + (slot + sub) * kKv4Head) + 16 * chunk;
+        uint8_t* out = reinterpret_cast<uint8_t*>(static_cast<__nv_bfloat16*>(P.attn.out) +
+                                                  sm.batch * P.attn.out_batch_stride +
+                                                  (long long)sm.head * P.group * kKv4Head) + 16 * chunk;
+        const int step = partial ? 32 : 64;                         // dims that make 128 bytes
 #pragma unroll 1
         for (int c0 = 0; ok && my_tiles > 0 && c0 < kKv4Head; c0 += step) {
             uint32_t o[32];
             KVP_TMEM_LD32(o_tm + c0, o);
             KVP_TMEM_WAIT_LD_DEP(o);
-            if (P.splits > 1) {
+            if (partial) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                     *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
@@ -478,17 +650,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             for (int i = 0; i < 8; ++i) {
                 const int k = 4 * i + sub;
                 const uint4 y = *reinterpret_cast<const uint4*>(stage + k * 128 + ((chunk ^ (k & 7)) << 4));
-                uint8_t* dst = P.splits > 1 ? ws + i * ws_step + c0 * 4
-                                            : out + (qi * P.attn.out_row_stride + qg * kKv4Head + c0) * 2;
+                uint8_t* dst = partial ? ws + i * (4 * kKv4Head * 4) + c0 * 4
+                                       : out + (qi * P.attn.out_row_stride + qg * kKv4Head + c0) * 2;
                 if (rw + k < er) *reinterpret_cast<uint4*>(dst) = y;
-                if (P.splits == 1)
+                if (!partial)
                     for (qg += 4; qg >= P.group; qg -= P.group) ++qi;
             }
             __syncwarp();
         }
+            done(P, sm, w);
+        }
     }
-    tc_fence_before();
-    __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
