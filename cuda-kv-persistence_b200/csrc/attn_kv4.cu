@@ -14,12 +14,14 @@
 #include "attn_kv4.cuh"
 #include "kernels.h"
 #include "kv4.h"
+#include "sm100_ptx.h"
 
 namespace kvp {
 
 namespace {
 
 using namespace kv4_dev;
+using ptx::pack_f16;
 
 // ------------------------------------------------- few query rows: mma.sync
 // Bound by the cache's bytes: 144 a key and K/V head, against 2 * 128 * 2
@@ -36,12 +38,18 @@ constexpr int kDecThreads = kWarps * 32;
 constexpr int kKeys = 32;                      // keys of one step of a warp
 constexpr float kRise = 8.f;                   // how far a score may pass the running max, log2 units
 
+// d += A B: bf16 (K Q^T) or fp16 (V^T P^T)
+template <bool kHalf>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if (kHalf)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -53,11 +61,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return reinterpret_cast<const uint32_t&>(h);
-}
-
 template <int NB>
 struct RowsSmem {
     float o[kWarps][8 * NB][kKv4Head];
@@ -205,8 +208,8 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
                     const uint32_t a6 = field<3>(k0[w], s0), a7 = field<3>(k1[w], s1);
 #pragma unroll
                     for (int i = 0; i < NB; ++i) {
-                        mma16816(c[i][e], a0, a1, a2, a3, qf[i][4 * w], qf[i][4 * w + 1]);
-                        mma16816(c[i][e], a4, a5, a6, a7, qf[i][4 * w + 2], qf[i][4 * w + 3]);
+                        mma16816<false>(c[i][e], a0, a1, a2, a3, qf[i][4 * w], qf[i][4 * w + 1]);
+                        mma16816<false>(c[i][e], a4, a5, a6, a7, qf[i][4 * w + 2], qf[i][4 * w + 3]);
                     }
                 }
             }
@@ -229,8 +232,7 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
                 }
         }
         // The max moves only when some score passes it by more than 2^8 (or a
-        // row sees its first key): P then stays below 2^8, far inside fp32 and
-        // bf16, and most steps need no reduction over the keys.
+        // row sees its first key): P then stays below 2^15, inside fp16, and most steps need no reduction over the keys.
         bool rise = false;
 #pragma unroll
         for (int i = 0; i < NB; ++i)
@@ -262,17 +264,17 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
         uint32_t p[NB][4];
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const float na0 = m[i][0] == -INFINITY ? 0.f : -m[i][0] * P.scale_log2;
-            const float na1 = m[i][1] == -INFINITY ? 0.f : -m[i][1] * P.scale_log2;
+            const float na0 = m[i][0] == -INFINITY ? 0.f : kPShift - m[i][0] * P.scale_log2;
+            const float na1 = m[i][1] == -INFINITY ? 0.f : kPShift - m[i][1] * P.scale_log2;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float p0 = ex2(fmaf(c[i][e >> 1][2 * (e & 1)], P.scale_log2, na0));
                 const float p1 = ex2(fmaf(c[i][e >> 1][2 * (e & 1) + 1], P.scale_log2, na1));
                 l[i][0] += p0;
                 l[i][1] += p1;
-                // P to bf16 (a tensor-core operand): at most 2^-8 of each
-                // weight, without bias; the sum l keeps 32 bits
-                p[i][e] = transpose8(pack2(p0, p1));
+                // P to fp16 (a tensor-core operand): off by 2^-11 of itself at
+                // most, or 2^-32 of the largest; the sum l keeps 32 bits
+                p[i][e] = transpose8(pack_f16(p0, p1));
             }
         }
         // O^T: word d of a row holds dims 16g + 8d + 2i (low half's field i)
@@ -281,8 +283,8 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const uint4 v0 = vc[2 * e], v1 = vc[2 * e + 1];
-            const Scale2 s0 = scale2(__byte_perm(vs[2 * e], 0, 0x4140));
-            const Scale2 s1 = scale2(__byte_perm(vs[2 * e + 1], 0, 0x4140));
+            const VScale2 s0 = vscale2(__byte_perm(vs[2 * e], 0, 0x4140));
+            const VScale2 s1 = vscale2(__byte_perm(vs[2 * e + 1], 0, 0x4140));
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
                 const uint32_t e0 = __byte_perm(d ? v0.y : v0.x, d ? v0.w : v0.z, 0x5410);
@@ -291,12 +293,12 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
                 const uint32_t o1 = __byte_perm(d ? v1.y : v1.x, d ? v1.w : v1.z, 0x7632);
                 auto step = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-                    for (int i = 0; i < NB; ++i) mma16816(o[i][j], a0, a1, a2, a3, p[i][2 * e], p[i][2 * e + 1]);
+                    for (int i = 0; i < NB; ++i) mma16816<true>(o[i][j], a0, a1, a2, a3, p[i][2 * e], p[i][2 * e + 1]);
                 };
-                step(4 * d, field<0>(e0, s0), field<0>(o0, s0), field<0>(e1, s1), field<0>(o1, s1));
-                step(4 * d + 1, field<1>(e0, s0), field<1>(o0, s0), field<1>(e1, s1), field<1>(o1, s1));
-                step(4 * d + 2, field<2>(e0, s0), field<2>(o0, s0), field<2>(e1, s1), field<2>(o1, s1));
-                step(4 * d + 3, field<3>(e0, s0), field<3>(o0, s0), field<3>(e1, s1), field<3>(o1, s1));
+                step(4 * d, vfield<0>(e0, s0), vfield<0>(o0, s0), vfield<0>(e1, s1), vfield<0>(o1, s1));
+                step(4 * d + 1, vfield<1>(e0, s0), vfield<1>(o0, s0), vfield<1>(e1, s1), vfield<1>(o1, s1));
+                step(4 * d + 2, vfield<2>(e0, s0), vfield<2>(o0, s0), vfield<2>(e1, s1), vfield<2>(o1, s1));
+                step(4 * d + 3, vfield<3>(e0, s0), vfield<3>(o0, s0), vfield<3>(e1, s1), vfield<3>(o1, s1));
             }
         }
         if (more) load_v(np);
@@ -319,7 +321,8 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
 #pragma unroll
             for (int j = 0; j < 8; j += 2)
                 *reinterpret_cast<float4*>(&sm.o[warp][q][16 * g + 2 * j]) =
-                    make_float4(o[i][j][a], o[i][j][a + 2], o[i][j + 1][a], o[i][j + 1][a + 2]);
+                    make_float4(o[i][j][a] * kVUnit, o[i][j][a + 2] * kVUnit, o[i][j + 1][a] * kVUnit,
+                                o[i][j + 1][a + 2] * kVUnit);
         }
     __syncthreads();
     for (int e = threadIdx.x; e < 8 * NB * (kKv4Head / 4); e += kDecThreads) {

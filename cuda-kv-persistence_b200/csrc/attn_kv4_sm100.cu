@@ -1,5 +1,5 @@
 // Attention over the 4-bit K/V cache for many query rows: tcgen05 tensor
-// cores, the cache expanded to bf16 on its way into shared memory.
+// cores, the cache expanded to 16 bits on its way into shared memory.
 //
 // Bound by the two products: 4 * 128 flops a (query row, key), against 144
 // bytes a key that every 256 query rows read again from L2.  CTA = two
@@ -8,7 +8,7 @@
 // other (Kv4Unit).  Warp roles (384 threads):
 //   warps 0, 2, 3   expand the cache: units of 32 rows of K or V in turn,
 //                   16-byte words from global memory (one unit ahead), fields
-//                   to bf16 in registers, 16-byte stores into the 128B-
+//                   to bf16 (K) and fp16 (V) in registers, 16-byte stores into the 128B-
 //                   swizzled tiles that TMA would write from bf16 rows (K
 //                   K-major, V MN-major); the words of half the lanes change
 //                   places so that no store conflicts
@@ -41,7 +41,7 @@ constexpr uint32_t kPanel = 128 * 128;        // one [128 rows][64 bf16] swizzle
 constexpr uint32_t kTileBytes = 2 * kPanel;
 constexpr int kRegsLow = 104, kRegsHigh = 200;   // warps 0-3, 4-11
 static_assert(kRegsLow * 128 + 2 * kRegsHigh * 128 <= 65536, "register split exceeds the SM");
-constexpr float kRedoSum = 256.f;             // a tile row sum above this takes the new max
+constexpr float kRedoSum = 32768.f;           // a tile row sum above this (2^8 shifted by kPShift) takes the new max
 constexpr int kUnits = 8;                     // of a tile: K rows 0-31, 32-63, .., then V's
 constexpr int kExpanders = 3;
 
@@ -100,7 +100,7 @@ __device__ __forceinline__ float exp_visible(uint32_t s_addr, float m, float sl2
             const float p1 = ex2_approx(fmaf(__uint_as_float(y[c + 1]), sl2, -m));
             part[0] += p0;
             part[1] += p1;
-            pk[16 * h + (c >> 1)] = pack_bf16(p0, p1);
+            pk[16 * h + (c >> 1)] = pack_f16(p0, p1);
         }
         sum += part[0] + part[1];
     }
@@ -129,6 +129,14 @@ __device__ __forceinline__ void expand4(uint8_t* tile, const uint32_t (&off)[4],
     *reinterpret_cast<uint4*>(tile + off[1]) = make_uint4(field<0>(w1, s01), field<1>(w1, s01), field<2>(w1, s01), field<3>(w1, s01));
     *reinterpret_cast<uint4*>(tile + off[2]) = make_uint4(field<0>(w2, s23), field<1>(w2, s23), field<2>(w2, s23), field<3>(w2, s23));
     *reinterpret_cast<uint4*>(tile + off[3]) = make_uint4(field<0>(w3, s23), field<1>(w3, s23), field<2>(w3, s23), field<3>(w3, s23));
+}
+
+__device__ __forceinline__ void expand4_v(uint8_t* tile, const uint32_t (&off)[4], uint32_t w0, uint32_t w1,
+                                          uint32_t w2, uint32_t w3, const VScale2& s01, const VScale2& s23) {
+    *reinterpret_cast<uint4*>(tile + off[0]) = make_uint4(vfield<0>(w0, s01), vfield<1>(w0, s01), vfield<2>(w0, s01), vfield<3>(w0, s01));
+    *reinterpret_cast<uint4*>(tile + off[1]) = make_uint4(vfield<0>(w1, s01), vfield<1>(w1, s01), vfield<2>(w1, s01), vfield<3>(w1, s01));
+    *reinterpret_cast<uint4*>(tile + off[2]) = make_uint4(vfield<0>(w2, s23), vfield<1>(w2, s23), vfield<2>(w2, s23), vfield<3>(w2, s23));
+    *reinterpret_cast<uint4*>(tile + off[3]) = make_uint4(vfield<0>(w3, s23), vfield<1>(w3, s23), vfield<2>(w3, s23), vfield<3>(w3, s23));
 }
 
 constexpr int kMinPages = 4;                  // of a CTA's share: a piece costs about three pages more
@@ -379,8 +387,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                     const bool swap = g & 1;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const Scale2 s0 = scale2(__byte_perm(ss[i], 0, 0x4040)), s1 = scale2(__byte_perm(ss[i], 0, 0x4141));
-                        expand4(tile + i * 1024, voff, swap ? cc[i].y : cc[i].x, swap ? cc[i].x : cc[i].y,
+                        const VScale2 s0 = vscale2(__byte_perm(ss[i], 0, 0x4040)), s1 = vscale2(__byte_perm(ss[i], 0, 0x4141));
+                        expand4_v(tile + i * 1024, voff, swap ? cc[i].y : cc[i].x, swap ? cc[i].x : cc[i].y,
                                 swap ? cc[i].w : cc[i].z, swap ? cc[i].z : cc[i].w, s0, s1);
                     }
                 } else {
@@ -401,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             // ============================ MMA issuer ==========================
             if (lane == 0) {
                 constexpr uint32_t idS = idesc_bf16(false);
-                constexpr uint32_t idO = idesc_bf16(true);
+                constexpr uint32_t idO = idesc_f16(true);
                 constexpr uint64_t kStageDesc = kTileBytes >> 4;
                 const uint64_t dq0 = sw128_desc(smem_u32(sm.q[0]), 16, 1024);
                 const uint64_t dq1 = sw128_desc(smem_u32(sm.q[1]), 16, 1024);
@@ -560,9 +568,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             for (int attempt = skip ? 1 : 0;; ++attempt) {
                 if ((attempt != 1 || !skip) && !all_gone) {
                     // (a row without keys keeps max -inf: subtract 0)
-                    const float mm = m_new == -INFINITY ? 0.f : m_new;
+                    const float mm = (m_new == -INFINITY ? 0.f : m_new) - kPShift;
                     rsum = masked ? exp_visible(s_tm, mm, P.scale_log2, vis, pk)
-                                  : exp_row<false, 4, 0u>(s_tm, mm, P.scale_log2, kBN, pk);
+                                  : exp_row<false, 4, 0u, true>(s_tm, mm, P.scale_log2, kBN, pk);
                 }
                 const bool redo = !gone && (skip ? attempt == 1 : attempt == 0 && !(rsum <= kRedoSum));
                 if (!__any_sync(0xffffffffu, redo)) break;
@@ -590,8 +598,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                     KVP_TMEM_ST32(o_tm + 32 * c4, o);
                 }
             }
-            // P (bf16: at most 2^-8 of each weight, without bias; the sum keeps
-            // 32 bits) -> the first 64 columns of S_q, key 2c in the low half
+            // P (fp16: off by 2^-11 of itself at most, or 2^-32 of the largest; the
+            // sum keeps 32 bits) -> the first 64 columns of S_q, key 2c in the low half
             KVP_TMEM_ST32(s_tm, pk);
             KVP_TMEM_ST32(s_tm + 32, (pk + 32));
             tmem_wait_st();
@@ -606,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
         tc_fence_after();
         uint8_t* stage = sm.q[qt] + (warp & 3) * 32 * 128;
         const int rw = r - lane, sub = lane >> 3, chunk = lane & 7;
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;         // a row without keys is 0
+        const float inv = l_run == 0.f ? 0.f : kVUnit / l_run;      // a row without keys is 0
         // row rw + sub + 4 i of the workspace or of the output
         const long long slot = unit_slot((int)blockIdx.x, sm.u0 == 0) * 256 + 128 * qt + (warp & 3) * 32;
         if (partial && ok && active)
@@ -625,7 +633,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                     *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                        make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                        make_uint4(__float_as_uint(__uint_as_float(o[4 * c]) * kVUnit),
+                                   __float_as_uint(__uint_as_float(o[4 * c + 1]) * kVUnit),
+                                   __float_as_uint(__uint_as_float(o[4 * c + 2]) * kVUnit),
+                                   __float_as_uint(__uint_as_float(o[4 * c + 3]) * kVUnit));
             } else {
 #pragma unroll 1
                 for (int e = 0; e < 2; ++e) {

@@ -76,11 +76,14 @@ __device__ __forceinline__ void tc_gemm_ts_tail(uint32_t d_tmem, uint32_t a_tmem
         ::"r"(d_tmem), "r"(a_tmem), "l"(b0), "r"(idesc));
 }
 
-// kind::f16 instruction descriptor: bf16 x bf16 -> f32, M=128, N=128.
+// kind::f16 instruction descriptors: bf16 x bf16 -> f32 and fp16 x fp16 -> f32,
+// M=128, N=128.
 constexpr uint32_t idesc_bf16(bool b_mn_major) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) |
            ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
+
+constexpr uint32_t idesc_f16(bool b_mn_major) { return idesc_bf16(b_mn_major) & ~((1u << 7) | (1u << 10)); }
 
 }  // namespace attn_dev
 }  // namespace kvp

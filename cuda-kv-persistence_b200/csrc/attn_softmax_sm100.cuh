@@ -83,8 +83,8 @@ __device__ __forceinline__ void ex2_poly2(float x0, float x1, float& y0, float& 
 // past `left` are masked (-inf) when kMask.  One exponential in eight runs
 // on the FMA pipe (ex2_poly2; the pairs of kPoly), the rest on MUFU, whose
 // 2^-inf is 0 where ex2_poly2's is not; scaling and the row sum use f32x2
-// arithmetic.
-template <bool kMask, int kChunks = 4, uint32_t kPoly = kPolyPairs>
+// arithmetic.  kHalf: P as fp16 pairs.
+template <bool kMask, int kChunks = 4, uint32_t kPoly = kPolyPairs, bool kHalf = false>
 __device__ __forceinline__ float exp_row(uint32_t s_addr, float m, float sl2, int left,
                                          uint32_t (&pk)[16 * kChunks]) {
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
@@ -119,7 +119,7 @@ __device__ __forceinline__ float exp_row(uint32_t s_addr, float m, float sl2, in
                 p1 = ex2_approx(x1);
             }
             acc[(c >> 1) & 3] = f2_add(acc[(c >> 1) & 3], f2_pack(p0, p1));
-            pk[16 * h + (c >> 1)] = pack_bf16(p0, p1);
+            pk[16 * h + (c >> 1)] = kHalf ? pack_f16(p0, p1) : pack_bf16(p0, p1);
         }
         if (h < kChunks - 1) KVP_TMEM_WAIT_LD_DEP(nxt);
     }

@@ -5,14 +5,14 @@
 // codes c, value (c - 8) * s.  A scale byte eeeee mmm is s = (1 + m/8) *
 // 2^(e - 15): no zero, no infinity, no NaN, so any bytes decode to finite
 // numbers and a masked key can never spread a NaN.  (c - 8) has at most 3
-// significant bits and s has 4, so every value is exact in bf16: the tensor
-// cores see just what the cache stands for.
+// significant bits and s has 4, so every value is exact in bf16, and in fp16
+// once divided by 64: the tensor cores see just what the cache stands for.
 //
 // Writing: s = max|x| / 7 rounded to 4 significant bits (halves up), within
-// [2^-15, 122880]; c - 8 = x / s rounded to the nearest integer (halves away
-// from zero).  Rounding s moves max|x| / s to 7.4375 at most, so no value is
-// clipped.  fp32 rows are rounded to bf16 first.  NaN is stored as 0 and
-// |x| > 860160 = 7 * 122880 as that bound; both set KVP_STATUS_RANGE.
+// [2^-15, 3840] (bytes 0 to 215); c - 8 = x / s rounded to the nearest integer
+// (halves away from zero).  Rounding s moves max|x| / s to 7.4375 at most, so
+// no value is clipped.  fp32 rows are rounded to bf16 first.  NaN is stored
+// as 0 and |x| > 26880 = 7 * 3840 as that bound; both set KVP_STATUS_RANGE.
 //
 // Layout.  Pages of 128 rows, uint8 [n_pages][kv_heads][18432]; a head's
 // share of a page is 16 blocks of 8 rows, each 1152 bytes: K codes [8 rows]
@@ -40,7 +40,8 @@ constexpr int kKv4PageHeadBytes = 16 * kKv4BlockBytes;    // 18432
 constexpr int kKv4KScale = 512;                           // offsets inside a block
 constexpr int kKv4VCode = 576;
 constexpr int kKv4VScale = 1088;
-constexpr float kKv4Top = 860160.f;                       // 7 * 1.875 * 2^16
+constexpr float kKv4Top = 26880.f;                        // 7 * 1.875 * 2^11
+constexpr int kKv4TopScale = 215;                         // the scale byte of 1.875 * 2^11
 constexpr int kKv4MaxRows = 1 << 30;                      // positions of a sequence stay below
 
 // Which rows of a cache a call touches: row i < count of sequence b is
@@ -130,6 +131,49 @@ __device__ __forceinline__ uint32_t field(uint32_t w, const Scale2& s) {
     uint32_t x;   // one lop3: (w & mask) | one
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> (4 * i)), "r"(0x000F000Fu), "r"(0x3F803F80u));
     return bf2_fma(x, s.hi, s.lo);
+}
+
+// V in fp16, as V / 64 (kVUnit): its ten mantissa bits take two codes without
+// a shift (0x3C00 | c is 1 + c/1024, 0x3C00 | c << 4 is 1 + c/64), so a word
+// needs one shift instead of three, and P in fp16 keeps eleven bits.  With s' =
+// s / 64, hi = 1024 s' and lo = -1032 s' = -(129/128) hi, hi4 = 64 s' and lo4 =
+// -72 s': at most 11 significant bits, between 2^-24 and 61920 for bytes up
+// to 215, all exact, and so is (c - 8) s'.  Higher bytes, which only unwritten
+// rows can hold, count as 215 so that they stay finite.
+//
+// P is 2^(x - m + kPShift) where a score passes the running max m by 8 at most: up to 2^15,
+// and fp16's floor of 2^-25 lies 2^-32 below the largest weight.  The sum l
+// holds the same factor, which cancels in O / l.
+constexpr float kVUnit = 64.f;
+constexpr float kPShift = 7.f;
+
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+struct VScale2 {
+    uint32_t hi, lo, hi4, lo4;
+};
+__device__ __forceinline__ VScale2 vscale2(uint32_t b2) {
+    VScale2 r;
+    r.hi = __vminu2(b2, 0x00D700D7u) * 128u + 0x10001000u;
+    r.lo = h2_mul(r.hi, 0xBC08BC08u);    // -129/128
+    r.hi4 = h2_mul(r.hi, 0x2C002C00u);   // 1/16
+    r.lo4 = h2_mul(r.hi, 0xAC80AC80u);   // -72/1024
+    return r;
+}
+template <int i>
+__device__ __forceinline__ uint32_t vfield(uint32_t w, const VScale2& s) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;"
+        : "=r"(x) : "r"(i < 2 ? w : w >> 8), "r"(i % 2 ? 0x00F000F0u : 0x000F000Fu), "r"(0x3C003C00u));
+    return i % 2 ? h2_fma(x, s.hi4, s.lo4) : h2_fma(x, s.hi, s.lo);
 }
 
 }  // namespace kv4_dev

@@ -114,7 +114,7 @@ __device__ __forceinline__ uint32_t quantise16(uint32_t (&x)[8], uint32_t (&word
         }
     }
     const uint32_t q = __float_as_uint(__fdiv_rn(top, 7.f)) + 0x80000u;   // halves up, at 4 bits
-    const int code = min(max((int)(q >> 20) - 896, 0), 255);              // 896 = (127 - 15) << 3
+    const int code = min(max((int)(q >> 20) - 896, 0), kKv4TopScale);              // 896 = (127 - 15) << 3
     const float s = __uint_as_float((uint32_t)(code + 896) << 20);
     const float r = __frcp_rn(s) * (1.f + 0x1p-14f);
 #pragma unroll

@@ -354,7 +354,7 @@ typedef struct {
 
 long long kvp_kv4_page_bytes(int kv_heads);
 
-/* Quantises the rows into the cache.  NaN is stored as 0 and |x| > 860160 as
+/* Quantises the rows into the cache.  NaN is stored as 0 and |x| > 26880 as
  * that bound; either sets status bit 3. */
 int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream);
 

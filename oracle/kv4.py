@@ -16,7 +16,8 @@ import torch
 
 PAGE, HEAD, PAGE_HEAD, BLOCK = 128, 128, 18432, 1152
 SCALES = np.array([(1 + m / 8) * 2.0 ** (e - 15) for e in range(32) for m in range(8)])
-TOP = 7 * SCALES[-1]
+TOP_BYTE = 215                                   # the largest scale that is written
+TOP = 7 * SCALES[TOP_BYTE]
 
 
 def bf16(x: np.ndarray) -> np.ndarray:
@@ -30,7 +31,8 @@ def quantise(x: np.ndarray):
     g = x.reshape(*x.shape[:-1], 8, 16)
     want = np.abs(g).max(-1) / 7
     # nearest scale, the upper one half-way (want * 7 and the bounds are exact)
-    middle = (SCALES[1:] + SCALES[:-1]) / 2 * 7
+    s = SCALES[: TOP_BYTE + 1]
+    middle = (s[1:] + s[:-1]) / 2 * 7
     byte = np.searchsorted(middle, np.abs(g).max(-1), side="right")
     assert byte.shape == want.shape
     r = np.abs(g) / SCALES[byte][..., None]            # exact enough: halves are exact quotients
@@ -92,8 +94,10 @@ def attention(q, k, v, ok):
     """q [rows, heads, 128], k / v [keys, kv_heads, 128], ok bool [rows, keys]
     -> out [rows, heads, 128] and a bound on |kernel - out|.
 
-    The bound counts a kernel's roundings: every weight to bf16 (2^-8 of it),
-    the result to bf16 (2^-8), the scores' fp32 sums of 128 products (each
+    The bound counts a kernel's roundings: every weight to 16 bits (bf16: 2^-8
+    of it; fp16 with the largest at 2^7 or above: 2^-11 of it, or half of its
+    smallest step of 2^-24, which is 2^-25 / 2^7 = 2^-32 of the largest and so of
+    the sum of the weights, for every key: 2^-32 sum |v|), the result to bf16 (2^-8), the scores' fp32 sums of 128 products (each
     partial sum off by 2^-23 of the sum of magnitudes, so a weight by d =
     130 * 2^-23 * max sum |q k| / sqrt(128)), the exponent's argument and the
     exponential itself (2^-21 (1 + max |score|)); the weights enter numerator and
@@ -119,5 +123,6 @@ def attention(q, k, v, ok):
         mag = mag.amax(-1, keepdim=True) if mag.shape[1] else torch.zeros(rows, 1, dtype=torch.float64)
         d = 130 * 2.0 ** -23 * mag + 2.0 ** -21 * (1 + mag)
         out[:, h] = o
-        tol[:, h] = (2.0 ** -8 + 2 * d + 2.0 ** -14) * a * (1 + 2.0 ** -8) + 2.0 ** -8 * o.abs()
+        floor = 2.0 ** -32 * (ok.double() @ vv.abs())
+        tol[:, h] = (2.0 ** -8 + 2 * d + 2.0 ** -14) * a * (1 + 2.0 ** -8) + 2.0 ** -8 * o.abs() + floor
     return out.numpy(), tol.numpy()
