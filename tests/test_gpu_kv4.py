@@ -265,6 +265,12 @@ ATTN = [  # batch, kv_heads, group, start, rows, options
     (1, 1, 1, 0, 300, dict(tokens=1000)),                       # one frame, not complete
     (1, 2, 1, 1560, 1560, dict(tokens=1560)),
     (1, 1, 3, 0, 700, dict(tokens=7, window=20, sinks=2)),
+    # splits: in a cluster, over the workspace (few, many, 9 to 16 rows)
+    (1, 4, 1, 2500, 1, {}), (1, 1, 1, 9000, 1, {}), (1, 1, 12, 9000, 1, {}), (1, 2, 3, 9000, 2, dict(window=6000, sinks=100)),
+    (48, 2, 1, 4200, 1, {}),
+    # units cut between CTAs: one unit for all of them, several, masked pages at the cuts
+    (1, 1, 1, 9000, 20, {}), (1, 1, 1, 6000, 300, dict(tokens=100, window=20, sinks=3)), (2, 3, 1, 2000, 400, {}),
+    (1, 2, 2, 3000, 500, dict(window=900, sinks=130)), (1, 1, 4, 1500, 750, dict(tokens=250, window=5, sinks=1)),
 ]
 
 
@@ -275,6 +281,23 @@ def test_attention(batch, kvh, grp, start, rows, kw):
     pages = _calm_pool(rng, batch * per + 1, kvh)
     m = _map(rng, batch, per, batch * per + 1)
     _check(*_attend(rng, pages, m, [start] * batch, [rows] * batch, rows, kvh * grp, **kw))
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_of_drawn_shapes(seed):
+    """Any batch, heads, rows, frames, window, sinks, starts and counts."""
+    rng = np.random.default_rng(1000 + seed)
+    kvh, grp, batch = int(rng.integers(1, 4)), int(rng.choice([1, 1, 2, 3, 5, 8])), int(rng.integers(1, 5))
+    rows = int(rng.choice([1, 1, 2, 3, 17, 40, 129, 260, 400]))
+    per = int(rng.integers(-(-rows // 128), 12))
+    T = int(rng.choice([1, 1, 7, 60, 128, 300]))
+    kw = dict(tokens=T, window=int(rng.choice([0, 1, 2, 5, 40])) * int(rng.choice([1, 1, 9])), sinks=int(rng.integers(0, 3)))
+    starts = [int(rng.integers(0, per * 128 - rows + 1)) for _ in range(batch)]
+    counts = [int(rng.integers(0, rows + 1)) if rng.random() < 0.4 else rows for _ in range(batch)]
+    pages = _calm_pool(rng, batch * per + 1, kvh)
+    m = _map(rng, batch, per, batch * per + 1)
+    _check(*_attend(rng, pages, m, starts, counts, rows, kvh * grp, use=("starts", "counts"), **kw))
     assert _status() == 0
 
 
@@ -307,7 +330,7 @@ def test_refused_sequences_are_left_alone(rows):
             assert bool((out[b] == 7).all()) != fits
 
 
-@pytest.mark.parametrize("rows,start", [(1, 600), (150, 450)])
+@pytest.mark.parametrize("rows,start", [(1, 600), (150, 450), (1, 9000), (150, 3450)])
 def test_bad_pages_are_no_keys(rows, start):
     rng = np.random.default_rng(5)
     per = -(-(start + rows) // 128)
@@ -428,14 +451,14 @@ def test_strided_queries_and_the_same_call_twice(rows, heads):
     assert bool((a[..., heads * 128:] == 7).all())
 
 
-@pytest.mark.parametrize("rows", [1, 130])
-def test_graphs_replay_and_do_not_share_workspaces(rows):
+@pytest.mark.parametrize("rows,far", [(1, 0), (1, 6000), (130, 0), (130, 3000)])
+def test_graphs_replay_and_do_not_share_workspaces(rows, far):
     """Two captured calls replayed at once on two streams, starts moved between replays."""
     from kvp import kv4
     rng = np.random.default_rng(15)
-    pages = torch.from_numpy(_calm_pool(rng, 32, 2)).cuda()
+    pages = torch.from_numpy(_calm_pool(rng, 32 + far // 128, 2)).cuda()
     qs = [torch.from_numpy(rng.standard_normal((1, rows, 512)).astype(np.float32)).to(BF).cuda() for _ in range(2)]
-    starts = [torch.tensor([1500 + 300 * i], dtype=torch.int32, device="cuda") for i in range(2)]
+    starts = [torch.tensor([1500 + far + 300 * i], dtype=torch.int32, device="cuda") for i in range(2)]
     outs = [torch.zeros_like(q) for q in qs]
     graphs = []
     for q, st, o in zip(qs, starts, outs):
