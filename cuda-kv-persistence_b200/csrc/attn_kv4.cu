@@ -449,22 +449,44 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(const Kv4Params P) {
 }
 
 // The units of the kernel for many rows that lie in several CTAs' chunks
-// (Kv4Unit): kUnitCtas CTAs a unit, a warp a row at a time.
-constexpr int kUnitCtas = 16;
+// (Kv4Unit): P.join_ctas CTAs a unit, a warp a row at a time, or all eight
+// warps where a unit is in many pieces.
 __global__ void __launch_bounds__(256) attn_kv4_join_units_kernel(const Kv4Params P) {
-    const int unit = (int)(blockIdx.x / kUnitCtas), lane = threadIdx.x & 31;
+    __shared__ float4 part[8][32];
+    const int unit = (int)blockIdx.x / P.join_ctas, cta = (int)blockIdx.x % P.join_ctas;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Kv4Unit u = unit_of(P, unit / P.span.kv_heads);
     cudaGridDependencySynchronize();
     if (u.pages == 0) return;
     const int chunk = P.ws_unit[0], page = P.ws_unit[1 + unit], c0 = page / chunk;
     const int splits = (page + u.pages - 1) / chunk - c0 + 1;
     if (splits == 1) return;                          // its rows are finished
-    const int rows = min(u.rows - u.r0, 256);
-    for (int row = (int)(blockIdx.x % kUnitCtas) * 8 + ((int)threadIdx.x >> 5); row < rows; row += kUnitCtas * 8) {
+    const int rows = min(u.rows - u.r0, 256), h = unit % P.span.kv_heads;
+    auto add = [&](int row, int first, int step, float4& acc) {
+        return add_partials(
+            P, splits, first, step, lane, [&](int c) { return unit_slot(c0 + c, c == 0) * 256 + row; }, acc);
+    };
+    if (splits <= 8) {
+        for (int row = cta * 8 + warp; row < rows; row += P.join_ctas * 8) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float sum = add(row, 0, 1, acc);
+            store_out(P, u.b, h, u.r0 + row, 4 * lane, acc, sum);
+        }
+        return;
+    }
+    for (int row = cta; row < rows; row += P.join_ctas) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float sum = add_partials(
-            P, splits, 0, 1, lane, [&](int c) { return unit_slot(c0 + c, c == 0) * 256 + row; }, acc);
-        store_out(P, u.b, unit % P.span.kv_heads, u.r0 + row, 4 * lane, acc, sum);
+        const float sum = add(row, warp, 8, acc);
+        __syncthreads();                              // (the row before has been read)
+        part[warp][lane] = acc;
+        __syncthreads();
+        if (warp) continue;
+#pragma unroll
+        for (int c = 1; c < 8; ++c) {
+            const float4 y = part[c][lane];
+            acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+        }
+        store_out(P, u.b, h, u.r0 + row, 4 * lane, acc, sum);
     }
 }
 
@@ -554,16 +576,28 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     P.scale_log2 = 1.4426950408889634f / sqrtf((float)kKv4Head);
     P.rise = kRise / P.scale_log2;
 
-    // Up to 16 rows of a K/V head fit the N side of the mma.sync kernel.
-    const bool tiles = P.max_rows > 16;
+    // Keys that the rows of one tile can see, at most (starts on the device: the
+    // capacity's).
+    auto keys_of = [&](int tile_rows) {
+        const long long all = s.starts ? cap : (long long)s.start + s.rows;
+        return a.window ? std::min(all, tile_rows / P.group + 2 + (long long)a.tokens + P.window_rows + P.sink_rows)
+                        : all;
+    };
+    // Up to 16 rows of a K/V head fit the N side of the mma.sync kernel; more go
+    // through it 16 at a time as long as that is quicker.  It takes a thousand
+    // 16-row x 32-key steps in 1.5 us after 7 us, the tcgen05 kernel a thousand
+    // of 256 rows in 4.1 us after 17 (12 heads x 4064 keys, 64 rows: 17.8 us and
+    // 25.0; 2 x 8 heads x 9064 keys, 32 rows: 19.1 and 41.2, 64 rows: 31.1 and
+    // 42.1; 16 x 8 heads x 8064 keys, 32 rows: 96.5 and 154, 64 rows: 190 and 153).
+    const double heads_k = (double)s.batch * s.kv_heads / kKeys * 1e-3;
+    const bool tiles = P.max_rows > 16 &&
+                       7 + (P.max_rows + 15) / 16 * heads_k * keys_of(16) * 1.5 >
+                           17 + (P.max_rows + 255) / 256 * heads_k * keys_of(256) * 4.1;
     const int nb = P.max_rows > 8 ? 2 : 1, tile_rows = tiles ? 256 : 8 * nb;
     P.row_tiles = (P.max_rows + tile_rows - 1) / tile_rows;
     const long long units = (long long)s.batch * s.kv_heads * P.row_tiles;
     long long grid = units, slots = 0;   // slots: rows of the workspace
-    // Keys of a row tile, at most (starts on the device: the capacity's).
-    long long keys = s.starts ? cap : (long long)s.start + s.rows;
-    if (a.window)
-        keys = std::min(keys, tile_rows / P.group + 2 + (long long)a.tokens + P.window_rows + P.sink_rows);
+    const long long keys = keys_of(tile_rows);
     if (tiles) {
         // A CTA an SM takes one unit after the other.  Units that do not divide
         // evenly over the SMs are cut: the CTAs share all units' pages, which
@@ -575,6 +609,8 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
         if (P.chunked) {
             grid = sm_count();
             slots = 2 * 256 * grid;
+            // eight CTAs an SM, at least sixteen a unit (few units are in many pieces)
+            P.join_ctas = (int)std::max(16LL, std::min(128LL, 8 * sms / units));
         }
     } else {
         const int* at_once = nullptr;
@@ -633,7 +669,7 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
             // a few splits: one warp a row; many: eight share them
             const long long rows = slots / P.splits;
             const bool many = P.splits > 8;
-            cfg.gridDim = dim3((unsigned)(tiles ? units * kUnitCtas : many ? rows : (rows + 7) / 8));
+            cfg.gridDim = dim3((unsigned)(tiles ? units * P.join_ctas : many ? rows : (rows + 7) / 8));
             const cudaError_t e = tiles  ? cudaLaunchKernelEx(&cfg, attn_kv4_join_units_kernel, P)
                                   : many ? cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel<8>, P)
                                          : cudaLaunchKernelEx(&cfg, attn_kv4_join_kernel<1>, P);

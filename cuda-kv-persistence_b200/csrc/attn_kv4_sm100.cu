@@ -139,7 +139,7 @@ __device__ __forceinline__ void expand4_v(uint8_t* tile, const uint32_t (&off)[4
     *reinterpret_cast<uint4*>(tile + off[3]) = make_uint4(vfield<0>(w3, s23), vfield<1>(w3, s23), vfield<2>(w3, s23), vfield<3>(w3, s23));
 }
 
-constexpr int kMinPages = 4;                  // of a CTA's share: a piece costs about three pages more
+constexpr int kMinPages = 2;                  // of a CTA's share: a piece costs about three pages more
 
 __device__ __forceinline__ void init_barriers(Smem& sm) {
     for (int q = 0; q < 2; ++q) {
