@@ -141,9 +141,9 @@ __device__ __forceinline__ uint32_t field(uint32_t w, const Scale2& s) {
 // to 215, all exact, and so is (c - 8) s'.  Higher bytes, which only unwritten
 // rows can hold, count as 215 so that they stay finite.
 //
-// P is 2^(x - m + kPShift) where a score passes the running max m by 8 at most: up to 2^15,
-// and fp16's floor of 2^-25 lies 2^-32 below the largest weight.  The sum l
-// holds the same factor, which cancels in O / l.
+// P is 2^(x - m + kPShift), and a score passes the running max m by 8 at most:
+// up to 2^15, and fp16's floor of 2^-25 lies 2^-32 below the largest weight.
+// The sum l holds the same factor, which cancels in O / l.
 constexpr float kVUnit = 64.f;
 constexpr float kPShift = 7.f;
 

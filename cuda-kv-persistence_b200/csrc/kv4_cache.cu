@@ -1,9 +1,12 @@
 // Writing the 4-bit K/V cache and reading it back (format: kv4.h).
 //
 // Both are byte movement: 512 B of a bf16 row and head against 144 B in the
-// cache, every byte touched once.  A warp owns one 8-row block of one head;
-// consecutive warps take consecutive heads of the same rows, so a CTA's
-// global rows are contiguous.
+// cache, every byte touched once.  A warp owns one 8-row block of one head,
+// which is what a scale's 16 dims and a page's blocks both divide into, so no
+// two warps share a byte; consecutive warps take consecutive heads of the same
+// rows, so a CTA's global rows are contiguous.  At 32760 bf16 rows x 12 heads
+// (258 MB) a write takes 44.9 us and a read 47.1, 5.7 and 5.5 TB/s; one
+// frame's write (1560 rows) 4.2 us and a token's 2.9, which is a launch.
 #include "kernels.h"
 #include "kv4.h"
 
@@ -132,10 +135,9 @@ __device__ __forceinline__ uint32_t quantise16(uint32_t (&x)[8], uint32_t (&word
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) kv4_write_kernel(const Kv4Span s, const T* __restrict__ k,
-                                                             const T* __restrict__ v, long long row_stride,
-                                                             long long batch_stride, int blocks,
-                                                             long long items, int* status) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
+    kv4_write_kernel(const Kv4Span s, const T* __restrict__ k, const T* __restrict__ v, long long row_stride,
+                     long long batch_stride, int blocks, long long items, int* status) {
     __shared__ __align__(16) uint8_t stage[sizeof(T) == 4 ? kThreads / 32 : 1][4096];
     const int lane = threadIdx.x & 31;
     const long long step = (long long)gridDim.x * (kThreads / 32);
@@ -291,6 +293,17 @@ int check_span(const char* who, const Kv4Span& s) {
     return KVP_OK;
 }
 
+// The rows of an output, `len` elements each, lie apart: sequence by sequence
+// or, row by row, with the sequences inside (the strides of a single row or
+// sequence mean nothing).
+bool apart(const Kv4Span& s, long long row_stride, long long batch_stride, long long len) {
+    if (s.rows > 1 && row_stride < len) return false;
+    if (s.batch <= 1 || s.rows <= 0) return true;
+    if (batch_stride < len) return false;
+    return s.rows == 1 || batch_stride >= (s.rows - 1) * row_stride + len ||
+           row_stride >= (s.batch - 1) * batch_stride + len;
+}
+
 template <class K>
 int launch(const Kv4Span& s, cudaStream_t stream, K&& kernel) {
     // rows may begin anywhere in a block: the last row's block is
@@ -324,9 +337,9 @@ int check_kv4_rows(const Kv4Span& s, const Kv4Rows& r, bool write) {
         set_error("%s: rows must be 16-byte aligned, strides too, and a row stride at least kv_heads * 128", who);
         return KVP_ERR_ARG;
     }
-    if (!write && s.batch > 1 && s.rows > 0 &&
-        r.batch_stride < (s.rows - 1) * r.row_stride + s.kv_heads * 128LL) {
-        set_error("kv4_read: the sequences' output rows overlap");
+    if (!write && s.rows > 0 && s.batch > 0 &&
+        (r.k == r.v || !apart(s, r.row_stride, r.batch_stride, s.kv_heads * 128LL))) {
+        set_error("kv4_read: the output rows overlap");
         return KVP_ERR_ARG;
     }
     return KVP_OK;
@@ -349,9 +362,8 @@ int check_kv4_attn(const Kv4Span& s, const Kv4Attn& a) {
         set_error("attn_kv4: q and out must be 16-byte aligned, strides multiples of 8 elements");
         return KVP_ERR_ARG;
     }
-    if ((s.rows > 1 && (a.q_row_stride < a.heads * 128LL || a.out_row_stride < a.heads * 128LL)) ||
-        (s.batch > 1 && s.rows > 0 &&
-         (a.q_batch_stride < 0 || a.out_batch_stride < (s.rows - 1) * a.out_row_stride + a.heads * 128LL))) {
+    if ((s.rows > 1 && a.q_row_stride < a.heads * 128LL) || (s.batch > 1 && a.q_batch_stride < 0) ||
+        !apart(s, a.out_row_stride, a.out_batch_stride, a.heads * 128LL)) {
         set_error("attn_kv4: strides overlap (a row is heads * 128 elements)");
         return KVP_ERR_ARG;
     }

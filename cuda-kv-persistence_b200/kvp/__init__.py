@@ -9,6 +9,7 @@ remapped attention path, over the C ABI of libkvp.so (include/*.h):
 * ``Session``            -- the per-frame KVMap loop of src/run_policy_experiment.cu:156-274
 * ``attn_forward_single_frame`` / ``attn_forward_launcher`` -- src/attn_kernel.h:15-29 (fp32)
 * ``attn_bf16``          -- the tcgen05 kernel (sm_100a)
+* ``kvp.kv4``            -- the 4-bit K/V cache: write, read, attention over it
 
 PyTorch tensors are used only as device memory and streams.
 """
@@ -18,4 +19,3 @@ from .layout import TileLayout  # noqa: F401
 from .manager import KVTileManager, KVTM_ADMITTED, KVTM_INVALID, KVTM_REFUSED_BUDGET  # noqa: F401
 from .policies import POLICIES, select  # noqa: F401
 from .session import Session  # noqa: F401
-from . import kv4  # noqa: F401

@@ -451,6 +451,55 @@ def test_strided_queries_and_the_same_call_twice(rows, heads):
     assert bool((a[..., heads * 128:] == 7).all())
 
 
+@pytest.mark.parametrize("rows", [1, 3, 130])
+def test_sequences_inside_rows_in_place_and_shared_queries(rows):
+    """Row-major batches ([rows, batch, ...] seen as [batch, rows, ...]) in
+    writes, reads and attention; out = q; one q for all sequences."""
+    from kvp import kv4
+    rng = np.random.default_rng(rows)
+    host = _calm_pool(rng, 3 * 34, 2)
+
+    def draw(n, d):
+        return torch.from_numpy(rng.standard_normal((n, 3, d)).astype(np.float32)).to(BF).cuda().transpose(0, 1)
+
+    k, v, q = draw(rows, 256), draw(rows, 256), draw(rows, 512)
+    a, b = (torch.from_numpy(host).cuda() for _ in range(2))
+    kv4.write(a, k, v, start=4100)
+    kv4.write(b, k.contiguous(), v.contiguous(), start=4100)
+    assert torch.equal(a, b)
+    for dtype in (BF, F32):
+        x, y = (torch.empty(rows, 3, 256, dtype=dtype, device="cuda").transpose(0, 1) for _ in range(2))
+        w = [torch.empty(3, rows, 256, dtype=dtype, device="cuda") for _ in range(2)]
+        kv4.read(a, x, y, start=4100)
+        kv4.read(a, *w, start=4100)
+        assert torch.equal(x, w[0]) and torch.equal(y, w[1])
+    want = torch.empty(3, rows, 512, dtype=BF, device="cuda")
+    kv4.attn(q.contiguous(), a, want, heads=4, start=4100)
+    out = torch.empty(rows, 3, 512, dtype=BF, device="cuda").transpose(0, 1)
+    kv4.attn(q, a, out, heads=4, start=4100)
+    assert torch.equal(out, want)
+    one = q[:1].expand(3, rows, 512)
+    kv4.attn(one, a, out, heads=4, start=4100)
+    kv4.attn(one.contiguous(), a, want, heads=4, start=4100)
+    assert torch.equal(out, want)
+    mine = one.contiguous()
+    kv4.attn(mine, a, mine, heads=4, start=4100)
+    assert torch.equal(mine, want)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("kw", [dict(tokens=2 ** 31 - 1), dict(window=2 ** 31 - 1), dict(sinks=2 ** 31 - 1, window=1),
+                                dict(tokens=2 ** 31 - 1, window=2 ** 31 - 1, sinks=2 ** 31 - 1),
+                                dict(tokens=3, window=2 ** 31 - 1)])
+def test_options_at_their_ends(rows, kw):
+    """Frames, windows and sinks beyond anything cached hide nothing."""
+    rng = np.random.default_rng(rows)
+    got, want, tol = _attend(rng, _calm_pool(rng, 12, 1), _map(rng, 1, 12, 12), [1000], [rows], rows, 2, **kw)
+    _check(got, want, tol)
+    assert _status() == 0
+
+
 @pytest.mark.parametrize("rows,far", [(1, 0), (1, 6000), (130, 0), (130, 3000)])
 def test_graphs_replay_and_do_not_share_workspaces(rows, far):
     """Two captured calls replayed at once on two streams, starts moved between replays."""

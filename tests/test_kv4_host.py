@@ -68,6 +68,19 @@ def test_refuses_overlapping_outputs_and_missing_operands():
     assert L.kvp_attn_kv4(None, None, None) == ERR_ARG
 
 
+def test_refuses_outputs_that_overlap_in_either_order():
+    """Sequence by sequence, or row by row with the sequences inside, and nothing between."""
+    rows = dict(row_stride=3 * 256 - 8, batch_stride=256)       # 3 sequences of 100 rows
+    span = dict(batch=3, rows=100, page_map=0x20000)
+    assert _call("kvp_kv4_read", Kv4Rows, ROWS, span, dict(rows, batch_stride=248)) == ERR_ARG
+    assert _call("kvp_kv4_read", Kv4Rows, ROWS, span, rows) == ERR_ARG
+    assert b"overlap" in lib().kvp_last_error()
+    assert _call("kvp_kv4_read", Kv4Rows, ROWS, span, dict(v=ROWS["k"])) == ERR_ARG
+    assert b"overlap" in lib().kvp_last_error()
+    assert _call("kvp_attn_kv4", Kv4Attn, ATTN, span, dict(out_row_stride=3 * 512 - 8, out_batch_stride=512)) == ERR_ARG
+    assert b"overlap" in lib().kvp_last_error()
+
+
 @pytest.mark.parametrize("bad", [
     dict(heads=3), dict(heads=0), dict(tokens=0), dict(window=-1), dict(sinks=-1), dict(q=0),
     dict(out=0), dict(q=0x50002), dict(out=0x60008), dict(q_row_stride=516), dict(out_row_stride=508),
