@@ -152,8 +152,9 @@ def attn(q, pages, out, *, heads: int, page_map=None, start: int = 0, starts=Non
          tokens: int = 1, window: int = 0, sinks: int = 0, stream=None) -> None:
     """out = attention of query rows q (bf16) over the cache: the row at
     position p, in frame f = p // tokens, sees the cached rows up to the end of
-    its frame (and of this call's rows) that lie in the last `window` frames (0: all) or the
-    first `sinks` frames.  The call's own rows are keys: write them first."""
+    its frame (and of this call's rows) that lie in the last `window` frames
+    (0: all) or the first `sinks` frames.  The call's own rows are keys: write
+    them first.  out may be q."""
     n_pages, kv_heads = _pool(pages)
     b, n, qr, qb = _rows3(q, "q", _Q_TYPES, heads)
     ob, on, orow, obatch = _rows3(out, "out", _Q_TYPES, heads)

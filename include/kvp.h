@@ -18,8 +18,9 @@ const char* kvp_version(void);
 const char* kvp_last_error(void);
 
 /* Device status word written by the kernels: bit 0 = a KVMap entry pointed
- * outside the arena (the base row was read instead), bit 1 = a bounded
- * device wait expired, bit 3 = the 4-bit cache was given a value it cannot
+ * outside the arena (the base row was read instead), or a page, start or count
+ * of the 4-bit cache was out of range (below), bit 1 = a bounded device wait
+ * expired, bit 3 = the 4-bit cache was given a value it cannot
  * hold (kvp_kv4_write).  Synchronises `stream`, returns and clears it. */
 int kvp_read_status(void* stream);
 
@@ -320,8 +321,11 @@ int kvp_session_run_frames_batched(void* s, int f0, int nframes, const float* sc
  * page's row.  A sequence whose device start or count does not fit (start <
  * 0, count not in [0, rows], start + count > 128 * map_stride) sets status
  * bit 0 and is left alone, its outputs too; so are rows at and behind
- * its count.  No call allocates for its results or waits for the device;
- * the buffers belong to the current device. */
+ * its count.  A call queues its work on `stream` and does not wait for the
+ * device; the buffers belong to the current device.  The first call on a
+ * device allocates the status word: make it before any stream capture.
+ * Several calls may run at once, on one cache too unless they write rows that
+ * another one touches. */
 typedef struct {
     void* pages;
     const int* page_map;  /* device int32 [batch][map_stride], or NULL: pages sequence * map_stride + p */
@@ -358,15 +362,19 @@ long long kvp_kv4_page_bytes(int kv_heads);
  * that bound; either sets status bit 3. */
 int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream);
 
-/* The values the rows stand for (exact in bf16 and fp32). */
+/* The values the rows stand for (exact in bf16 and fp32).  Output rows must
+ * not overlap. */
 int kvp_kv4_read(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream);
 
 /* softmax(q K^T / sqrt(128)) V over the cache: query row i of a sequence, at
  * position p = start + i in frame f = p / tokens, sees the positions below
  * min((f + 1) * tokens, start + count) that are in frames f - window + 1 ..
  * f or in the first `sinks` frames.  (The call's own rows are keys too: write
- * them first.)  A row that sees no key is 0.  One row per sequence is a
- * decoding step, tokens = 1 a causal prompt, tokens = 1560 a video frame. */
+ * them first.)  A row that sees no key is 0; one of q that is not finite
+ * spoils its own output only.  out may be q, with the same strides.  One row
+ * per sequence is a decoding step, tokens = 1 a causal prompt, tokens = 1560 a
+ * video frame.  Keys that are split over several CTAs are joined through a
+ * workspace from the private, stream-ordered memory pool. */
 int kvp_attn_kv4(const kvp_kv4_span* s, const kvp_kv4_attn* a, void* stream);
 
 #ifdef __cplusplus
