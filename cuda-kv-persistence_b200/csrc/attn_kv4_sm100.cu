@@ -8,8 +8,8 @@
 // other (Kv4Unit).  Warp roles (384 threads):
 //   warps 0, 2, 3   expand the cache: units of 32 rows of K or V in turn,
 //                   16-byte words from global memory (one unit ahead), fields
-//                   to bf16 (K) and fp16 (V) in registers, 16-byte stores into the 128B-
-//                   swizzled tiles that TMA would write from bf16 rows (K
+//                   to bf16 (K) and fp16 (V) in registers, 16-byte stores into
+//                   the 128B-swizzled tiles that TMA would write from bf16 rows (K
 //                   K-major, V MN-major); the words of half the lanes change
 //                   places so that no store conflicts
 //   warp 1          TMEM and the single-thread MMA issuer: S0_j, PV1_{j-1},
@@ -19,6 +19,17 @@
 //                   overgrows
 // TMEM: S0 | S1 | O0 | O1, 128 columns each; P overlays S's first 64.
 // Every wait is bounded (sm100_ptx.h).
+//
+// One frame of 1560 rows over 32760 keys x 12 heads takes 380 us (827 TFLOP/s
+// of products that are needed, half of what a large bf16 GEMM reaches), three
+// frames with a window of six and the first one kept 411, a token-causal
+// prompt of 4097 rows x 24 heads with a window of 1024 99.  A page takes a CTA
+// about 4400 cycles, 2048 of them MMAs: a query tile's S, its softmax (2300
+// cycles while the other tile's warps run theirs) and its PV follow one
+// another, and the two tiles' softmax share the SM's issue slots and MUFU.
+// Expanding the cache costs 5 %.  Measured and slower: S in halves of 64 keys
+// that land under the other half's softmax (+22 %), two threads a row (+15 %);
+// part of the exponentials on the FMA pipes gave nothing.
 #include <cstring>
 
 #include "attn_kv4.cuh"
@@ -45,6 +56,18 @@ constexpr float kRedoSum = 32768.f;           // a tile row sum above this (2^8 
 constexpr int kUnits = 8;                     // of a tile: K rows 0-31, 32-63, .., then V's
 constexpr int kExpanders = 3;
 
+// Where a CTA is in its list of units, and the pages it still takes.  Each role
+// holds its own and moves it on by itself.
+struct Work {
+    int pair, head, off, left, pos;
+};
+
+// A piece for the softmax, which holds little of it in registers.
+struct Turn {
+    Work w;
+    volatile int batch, start, end, rows, row0, u0, n_tiles, rot, na, b0, two, partial, free_n, tile0;
+};
+
 struct __align__(1024) Smem {
     uint8_t q[2][kTileBytes];
     uint8_t k[kKStages][kTileBytes];
@@ -59,11 +82,9 @@ struct __align__(1024) Smem {
     uint32_t tmem_base;
     int abort_flag;
     int scan[kThreads / 32];
-    // The CTA's work list: what it does next (thread 0 moves it on).
-    volatile int pair, head, off, left, pos;
-    volatile int any_bad[2];    // a page of the piece is not in the pool; the other for the next piece
-    // The piece, for what the softmax seldom needs (not held in registers)
-    volatile int batch, rows, row0, u0, n_tiles, rot, na, b0, partial, releaser, free_n;
+    Work first;                 // where the CTA begins
+    volatile int bad[8];        // K/V tile i of the CTA: its page is not in the pool (slot i % 8)
+    Turn turn[2][2];            // [query tile][piece % 2]
 };
 
 // Bits [0, n) set.
@@ -122,21 +143,21 @@ __device__ __forceinline__ float max_visible(uint32_t s_addr, const uint32_t (&v
     return m;
 }
 
-// The four words and scale bytes of a lane's 16 bytes as four bf16 chunks.
-__device__ __forceinline__ void expand4(uint8_t* tile, const uint32_t (&off)[4], uint32_t w0, uint32_t w1,
-                                        uint32_t w2, uint32_t w3, const Scale2& s01, const Scale2& s23) {
-    *reinterpret_cast<uint4*>(tile + off[0]) = make_uint4(field<0>(w0, s01), field<1>(w0, s01), field<2>(w0, s01), field<3>(w0, s01));
-    *reinterpret_cast<uint4*>(tile + off[1]) = make_uint4(field<0>(w1, s01), field<1>(w1, s01), field<2>(w1, s01), field<3>(w1, s01));
-    *reinterpret_cast<uint4*>(tile + off[2]) = make_uint4(field<0>(w2, s23), field<1>(w2, s23), field<2>(w2, s23), field<3>(w2, s23));
-    *reinterpret_cast<uint4*>(tile + off[3]) = make_uint4(field<0>(w3, s23), field<1>(w3, s23), field<2>(w3, s23), field<3>(w3, s23));
+// A word's eight values, K in bf16 and V in fp16, and a lane's four words as
+// four 16-byte chunks of a tile.
+__device__ __forceinline__ uint4 values(uint32_t w, const Scale2& s) {
+    return make_uint4(field<0>(w, s), field<1>(w, s), field<2>(w, s), field<3>(w, s));
 }
-
-__device__ __forceinline__ void expand4_v(uint8_t* tile, const uint32_t (&off)[4], uint32_t w0, uint32_t w1,
-                                          uint32_t w2, uint32_t w3, const VScale2& s01, const VScale2& s23) {
-    *reinterpret_cast<uint4*>(tile + off[0]) = make_uint4(vfield<0>(w0, s01), vfield<1>(w0, s01), vfield<2>(w0, s01), vfield<3>(w0, s01));
-    *reinterpret_cast<uint4*>(tile + off[1]) = make_uint4(vfield<0>(w1, s01), vfield<1>(w1, s01), vfield<2>(w1, s01), vfield<3>(w1, s01));
-    *reinterpret_cast<uint4*>(tile + off[2]) = make_uint4(vfield<0>(w2, s23), vfield<1>(w2, s23), vfield<2>(w2, s23), vfield<3>(w2, s23));
-    *reinterpret_cast<uint4*>(tile + off[3]) = make_uint4(vfield<0>(w3, s23), vfield<1>(w3, s23), vfield<2>(w3, s23), vfield<3>(w3, s23));
+__device__ __forceinline__ uint4 values(uint32_t w, const VScale2& s) {
+    return make_uint4(vfield<0>(w, s), vfield<1>(w, s), vfield<2>(w, s), vfield<3>(w, s));
+}
+template <class S>
+__device__ __forceinline__ void expand4(uint8_t* tile, const uint32_t (&off)[4], uint32_t w0, uint32_t w1, uint32_t w2,
+                                        uint32_t w3, const S& s01, const S& s23) {
+    *reinterpret_cast<uint4*>(tile + off[0]) = values(w0, s01);
+    *reinterpret_cast<uint4*>(tile + off[1]) = values(w1, s01);
+    *reinterpret_cast<uint4*>(tile + off[2]) = values(w2, s23);
+    *reinterpret_cast<uint4*>(tile + off[3]) = values(w3, s23);
 }
 
 constexpr int kMinPages = 2;                  // of a CTA's share: a piece costs about three pages more
@@ -168,10 +189,10 @@ struct Piece {
     Kv4Unit u;
     int u0, n_tiles, rot;
     bool two;                                 // the second query tile has rows
-    __device__ __forceinline__ Piece(const Kv4Params& P, Smem& sm) {
-        u = unit_of(P, sm.pair);
-        u0 = sm.off;
-        n_tiles = min(u.pages - u0, sm.left);
+    __device__ __forceinline__ Piece(const Kv4Params& P, const Work& w) {
+        u = unit_of(P, w.pair);
+        u0 = w.off;
+        n_tiles = min(u.pages - u0, w.left);
         two = u.r0 + 128 < u.rows;
         rot = free0() < free1() ? free0() : 0;
     }
@@ -185,61 +206,43 @@ struct Piece {
         const int i = u0 + (j < n_tiles ? j : j - n_tiles);
         return i < u.na ? i : i - u.na + u.b0;
     }
-    // Every thread: the piece's pages are looked up once, the roles may start after it.
-    __device__ __forceinline__ void set_up(const Kv4Params& P, Smem& sm, int turn) const {
-        for (int j = threadIdx.x; j < n_tiles; j += kThreads)
-            if (page_of(P.span, u.b, page_pos(j)) < 0) sm.any_bad[turn & 1] = 1;
-        if (threadIdx.x == 0) {
-            sm.any_bad[(turn + 1) & 1] = 0;
-            sm.batch = u.b;
-            sm.rows = u.rows;
-            sm.row0 = u.r0;
-            sm.u0 = u0;
-            sm.n_tiles = n_tiles;
-            sm.rot = rot;
-            sm.na = u.na;
-            sm.b0 = u.b0;
-            sm.partial = n_tiles < u.pages;
-            sm.releaser = two ? 256 : 128;
-            sm.free_n = max(free1() - free0(), 0);
-            if (P.chunked && u0 == 0) P.ws_unit[1 + sm.pair * P.span.kv_heads + sm.head] = sm.pos;
-        }
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
-        if (sm.any_bad[turn & 1] && threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_MAP);
-    }
 };
 
-// Every thread: the piece is done; thread 0 moves the list on.
-__device__ __forceinline__ void done(const Kv4Params& P, Smem& sm, const Piece& w) {
-    tc_fence_before();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int pair = sm.pair, head = sm.head + 1;
-        const int left = sm.left - w.n_tiles;
-        if (left > 0 && head == P.span.kv_heads) {
-            head = 0;
-            do ++pair;
-            while (unit_of(P, pair).pages == 0);        // left > 0: there is one
-        }
-        sm.pair = pair;
-        sm.head = head;
-        sm.off = 0;
-        sm.pos = sm.pos + w.n_tiles;
-        sm.left = left;
-        if (left > 0) {
-            uint64_t* bars[] = {sm.bar_q, sm.bar_s_full, sm.bar_p_full, sm.bar_o_done, sm.bar_kfull, sm.bar_kempty,
-                                sm.bar_vfull, sm.bar_vempty, &sm.bar_mma_done};
-            const int n[] = {2, 2, 2, 2, kKStages, kKStages, kVStages, kVStages, 1};
-            for (int i = 0; i < 9; ++i)
-                for (int e = 0; e < n[i]; ++e)
-                    asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bars[i] + e)) : "memory");
-            init_barriers(sm);
-        }
+// The next piece of the list after one of n_tiles.
+__device__ __forceinline__ void advance(const Kv4Params& P, Work& w, int n_tiles) {
+    w.left -= n_tiles;
+    w.pos += n_tiles;
+    w.off = 0;
+    if (++w.head == P.span.kv_heads && w.left > 0) {
+        w.head = 0;
+        do ++w.pair;
+        while (unit_of(P, w.pair).pages == 0);        // left > 0: there is one
     }
-    __syncthreads();
-    tc_fence_after();
+}
+
+// A piece's entry for the softmax (tile0: the CTA's K/V tiles before it).
+__device__ __forceinline__ void describe(const Kv4Params& P, Turn& t, const Work& w, int first_pos) {
+    const Piece p(P, w);
+    t.w = w;
+    t.batch = p.u.b;
+    t.start = p.u.start;
+    t.end = p.u.end;
+    t.rows = p.u.rows;
+    t.row0 = p.u.r0;
+    t.u0 = p.u0;
+    t.n_tiles = p.n_tiles;
+    t.rot = p.rot;
+    t.na = p.u.na;
+    t.b0 = p.u.b0;
+    t.two = p.two;
+    t.partial = p.n_tiles < p.u.pages;
+    t.free_n = max(p.free1() - p.free0(), 0);
+    t.tile0 = w.pos - first_pos;
+}
+
+__device__ __forceinline__ void query_tile_sync(int qt) {     // its four warps
+    if (qt) asm volatile("bar.sync 2, 128;" ::: "memory");
+    else asm volatile("bar.sync 1, 128;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __grid_constant__ Kv4Params P) {
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
     const Kv4Span& s = P.span;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // Where this CTA's work begins, and how many pages it takes.
-    int pair = 0, head = 0, off = 0, left = 0, pos = 0;
+    int left = 0;
     if (P.chunked) {
         // prefix sums of the pairs' pages, three pairs a thread
         const int pairs = P.row_tiles * s.batch;
@@ -279,28 +282,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
         }
         all *= s.kv_heads;
         const int chunk = max((all + (int)gridDim.x - 1) / (int)gridDim.x, kMinPages);
-        pos = (int)min((long long)blockIdx.x * chunk, (long long)all);
+        const int pos = (int)min((long long)blockIdx.x * chunk, (long long)all);
         left = min(chunk, all - pos);
         if (blockIdx.x == 0 && threadIdx.x == 0) P.ws_unit[0] = chunk;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
             const int r = pos - before * s.kv_heads;   // pages into this pair's kv_heads units
             if (left > 0 && r >= 0 && r < n[i] * s.kv_heads) {
-                sm.pair = 3 * (int)threadIdx.x + i;
-                sm.head = r / n[i];
-                sm.off = r % n[i];
+                sm.first = Work{3 * (int)threadIdx.x + i, r / n[i], r % n[i], left, pos};
             }
             before += n[i];
         }
     } else {
-        pair = (int)(blockIdx.x / (uint32_t)s.kv_heads);
-        head = (int)(blockIdx.x % (uint32_t)s.kv_heads);
+        const int pair = (int)(blockIdx.x / (uint32_t)s.kv_heads);
         left = unit_of(P, pair).pages;
-        if (threadIdx.x == 0) {
-            sm.pair = pair;
-            sm.head = head;
-            sm.off = off;
-        }
+        if (threadIdx.x == 0) sm.first = Work{pair, (int)(blockIdx.x % (uint32_t)s.kv_heads), 0, left, 0};
     }
     // the refused sequences are reported once
     if (threadIdx.x == 0)
@@ -308,10 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             if (unit_of(P, i).refused) atomicOr(P.status, KVP_STATUS_MAP);
     if (left == 0) return;
     if (threadIdx.x == 0) {
-        sm.left = left;
-        sm.pos = pos;
         sm.abort_flag = 0;
-        sm.any_bad[0] = sm.any_bad[1] = 0;
         init_barriers(sm);
     }
     if (warp == 1) {
@@ -324,37 +317,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
 
-    // Both sides of the role split go through the same pieces, with the same
-    // three barriers for each.
+    // Every role goes through the pieces by itself; the barriers' phases run on
+    // from one to the next, so that the first tiles of a piece are expanded
+    // while the one before ends.
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
-        for (int turn = 0; sm.left > 0; ++turn) {
-            const Piece w(P, sm);
-            const int n_tiles = w.n_tiles, h = sm.head;
-            const bool two = w.two;
-            auto lookup = [&](int j) { return j < n_tiles ? page_of(s, w.u.b, w.page_pos(j)) : 0; };
-            const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
-            const uint8_t* pool = static_cast<const uint8_t*>(s.pages) + h * kKv4PageHeadBytes;
-            const int units = n_tiles * kUnits;
-            uint4 c[4];
-            uint32_t sc[4];
-            auto load = [&](int n, int page) {
-                const int part = (n >> 2) & 1;
-                const uint8_t* p = pool + (unsigned long long)(uint32_t)max(page, 0) * page_bytes +
-                                   (n & 3) * 4 * kKv4BlockBytes;
-                const uint8_t* pc = p + (part ? kKv4VCode : 0) + lane * 16;
-                const uint8_t* ps = p + (part ? kKv4VScale : kKv4KScale) + lane * 2;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    c[i] = *reinterpret_cast<const uint4*>(pc + i * kKv4BlockBytes);
-                    sc[i] = *reinterpret_cast<const uint16_t*>(ps + i * kKv4BlockBytes);
-                }
-            };
-            // an expander's unit of 32 rows; its first is on its way while the CTA sets up
-            int n = warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : units;
-            int page = lookup(n / kUnits), page1 = lookup((n + kExpanders) / kUnits);
-            if (n < units) load(n, page);
-            w.set_up(P, sm, turn);
+        Work w = sm.first;
         if (warp != 1) {
             // ============================ expanders ===========================
             const int g = lane >> 2, t = lane & 3;
@@ -367,43 +335,81 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 voff[i] = (g >> 2) * kPanel + (2 * t + (i >> 1)) * 128 +
                           ((((g & 3) * 2) ^ (g & 1) ^ (2 * t) ^ (i >> 1) ^ (i & 1)) << 4);
             }
-            for (; n < units; n += kExpanders) {
-                page = page1;
-                page1 = lookup((n + 2 * kExpanders) / kUnits);
-                uint4 cc[4];
-                uint32_t ss[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    cc[i] = c[i];
-                    ss[i] = sc[i];
-                }
-                if (n + kExpanders < units) load(n + kExpanders, page);
-                const int j = n / kUnits, part = (n >> 2) & 1;
-                const int st = part ? j % kVStages : j % kKStages;
-                const uint32_t ph = (uint32_t)(part ? j / kVStages : j / kKStages) & 1u;
-                if (!warp_wait(part ? &sm.bar_vempty[st] : &sm.bar_kempty[st], ph ^ 1u, sm, P.status)) break;
-                uint8_t* tile = (part ? sm.v[st] : sm.k[st]) + (n & 3) * 4 * 1024;   // 8 rows: 1024 bytes of a panel
-                if (part) {
-                    const bool swap = g & 1;
+            const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
+            const int turn0 = warp == 0 ? 0 : warp - 1;    // its first unit of a piece
+            bool ok = true;
+            for (int tile0 = 0; ok && w.left > 0;) {
+                const Piece pc(P, w);
+                const int units = pc.n_tiles * kUnits;
+                const uint8_t* pool = static_cast<const uint8_t*>(s.pages) + w.head * kKv4PageHeadBytes;
+                auto lookup = [&](int n) { return n < units ? page_of(s, pc.u.b, pc.page_pos(n / kUnits)) : 0; };
+                uint4 c[4];
+                uint32_t sc[4];
+                auto load = [&](int n, int page) {
+                    const int part = (n >> 2) & 1;
+                    const uint8_t* p = pool + (unsigned long long)(uint32_t)max(page, 0) * page_bytes +
+                                       (n & 3) * 4 * kKv4BlockBytes;
+                    const uint8_t* at = p + (part ? kKv4VCode : 0) + lane * 16;
+                    const uint8_t* ps = p + (part ? kKv4VScale : kKv4KScale) + lane * 2;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const VScale2 s0 = vscale2(__byte_perm(ss[i], 0, 0x4040)), s1 = vscale2(__byte_perm(ss[i], 0, 0x4141));
-                        expand4_v(tile + i * 1024, voff, swap ? cc[i].y : cc[i].x, swap ? cc[i].x : cc[i].y,
-                                swap ? cc[i].w : cc[i].z, swap ? cc[i].z : cc[i].w, s0, s1);
+                        c[i] = *reinterpret_cast<const uint4*>(at + i * kKv4BlockBytes);
+                        sc[i] = *reinterpret_cast<const uint16_t*>(ps + i * kKv4BlockBytes);
                     }
-                } else {
-                    const bool swap = t & 2;
-                    const uint32_t lo = swap ? 0x4141 : 0x4040, hi = swap ? 0x4040 : 0x4141;
+                };
+                int n = turn0, page = lookup(n), page1 = lookup(n + kExpanders);
+                load(n, page);
+                for (; n < units; n += kExpanders) {
+                    const bool bad = page < 0;
+                    page = page1;
+                    page1 = lookup(n + 2 * kExpanders);
+                    uint4 cc[4];
+                    uint32_t ss[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const Scale2 s0 = scale2(__byte_perm(ss[i], 0, lo)), s1 = scale2(__byte_perm(ss[i], 0, hi));
-                        expand4(tile + i * 1024, koff, swap ? cc[i].z : cc[i].x, swap ? cc[i].w : cc[i].y,
-                                swap ? cc[i].x : cc[i].z, swap ? cc[i].y : cc[i].w, s0, s1);
+                        cc[i] = c[i];
+                        ss[i] = sc[i];
                     }
+                    if (n + kExpanders < units) load(n + kExpanders, page);
+                    const int j = tile0 + n / kUnits, part = (n >> 2) & 1;
+                    const int st = part ? j % kVStages : j % kKStages;
+                    const uint32_t ph = (uint32_t)(part ? j / kVStages : j / kKStages) & 1u;
+                    if (!warp_wait(part ? &sm.bar_vempty[st] : &sm.bar_kempty[st], ph ^ 1u, sm, P.status)) {
+                        ok = false;
+                        break;
+                    }
+                    if (n % kUnits == 0 && lane == 0) {
+                        sm.bad[j % 8] = bad;
+                        if (bad) atomicOr(P.status, KVP_STATUS_MAP);
+                    }
+                    // 8 rows are 1024 bytes of a panel
+                    uint8_t* tile = (part ? sm.v[st] : sm.k[st]) + (n & 3) * 4 * 1024;
+                    if (part) {
+                        const bool swap = g & 1;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const VScale2 s0 = vscale2(__byte_perm(ss[i], 0, 0x4040));
+                            const VScale2 s1 = vscale2(__byte_perm(ss[i], 0, 0x4141));
+                            expand4(tile + i * 1024, voff, swap ? cc[i].y : cc[i].x, swap ? cc[i].x : cc[i].y,
+                                    swap ? cc[i].w : cc[i].z, swap ? cc[i].z : cc[i].w, s0, s1);
+                        }
+                    } else {
+                        const bool swap = t & 2;
+                        const uint32_t lo = swap ? 0x4141 : 0x4040, hi = swap ? 0x4040 : 0x4141;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const Scale2 s0 = scale2(__byte_perm(ss[i], 0, lo));
+                            const Scale2 s1 = scale2(__byte_perm(ss[i], 0, hi));
+                            expand4(tile + i * 1024, koff, swap ? cc[i].z : cc[i].x, swap ? cc[i].w : cc[i].y,
+                                    swap ? cc[i].x : cc[i].z, swap ? cc[i].y : cc[i].w, s0, s1);
+                        }
+                    }
+                    fence_proxy_async_smem();   // each lane's stores, before the arrival that covers them
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(part ? &sm.bar_vfull[st] : &sm.bar_kfull[st]);
                 }
-                fence_proxy_async_smem();   // each lane's stores, before the arrival that covers them
-                __syncwarp();
-                if (lane == 0) mbar_arrive(part ? &sm.bar_vfull[st] : &sm.bar_kfull[st]);
+                tile0 += pc.n_tiles;
+                advance(P, w, pc.n_tiles);
             }
         } else {
             // ============================ MMA issuer ==========================
@@ -416,58 +422,71 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 const uint64_t dk = sw128_desc(smem_u32(sm.k[0]), 16, 1024);
                 const uint64_t dv = sw128_desc(smem_u32(sm.v[0]), kPanel, 1024);
                 const uint32_t s0_tm = tmem, s1_tm = tmem + 128u, o0_tm = tmem + 256u, o1_tm = tmem + 384u;
-                bool ok = n_tiles > 0 && mbar_wait(&sm.bar_q[0], 0, sm, P.status);
-                if (ok && two) ok = mbar_wait(&sm.bar_q[1], 0, sm, P.status);
                 uint32_t ks = 0, kph = 0, vs = 0, vph = 0, pvs = 0;
-                bool k_known = false;
-                // While the first six MMAs of a GEMM are queued, the barriers of
-                // the next GEMM are tested without blocking.
-                for (int j = 0; ok && j < n_tiles; ++j) {
-                    if (!k_known && !(ok = mbar_wait(&sm.bar_kfull[ks], kph, sm, P.status))) break;
-                    tc_fence_after();
-                    const uint64_t kd = dk + ks * kStageDesc;
-                    const bool pv1 = two && j > 0;
-                    tc_gemm_ss_head(s0_tm, dq0, kd, idS);
-                    const bool pv1_ready = pv1 && mbar_test(&sm.bar_p_full[1], (uint32_t)(j - 1) & 1u);
-                    tc_gemm_ss_tail(s0_tm, dq0, kd, idS);
-                    tc_commit(&sm.bar_s_full[0]);
-                    if (pv1) {
-                        if (!pv1_ready && !(ok = mbar_wait(&sm.bar_p_full[1], (uint32_t)(j - 1) & 1u, sm, P.status))) break;
+                uint32_t q0_ph = 0, q1_ph = 0, p0_ph = 0, p1_ph = 0;
+                bool ok = true;
+                while (ok && w.left > 0) {
+                    const Piece pc(P, w);
+                    const int n_tiles = pc.n_tiles;
+                    const bool two = pc.two;
+                    ok = mbar_wait(&sm.bar_q[0], q0_ph, sm, P.status);
+                    if (ok && two) ok = mbar_wait(&sm.bar_q[1], q1_ph, sm, P.status);
+                    bool k_known = false;
+                    // While the first six MMAs of a GEMM are queued, the barriers of
+                    // the next GEMM are tested without blocking.
+                    for (int j = 0; ok && j < n_tiles; ++j) {
+                        if (!k_known && !(ok = mbar_wait(&sm.bar_kfull[ks], kph, sm, P.status))) break;
                         tc_fence_after();
-                        const uint64_t vd = dv + pvs * kStageDesc;
-                        tc_gemm_ts_head(o1_tm, s1_tm, vd, idO, j > 1 ? 1u : 0u);
-                        tc_gemm_ts_tail(o1_tm, s1_tm, vd, idO);
-                    }
-                    bool pv0_ready = false;
-                    if (two) {
-                        tc_gemm_ss_head(s1_tm, dq1, kd, idS);
-                        pv0_ready = mbar_test(&sm.bar_vfull[vs], vph) && mbar_test(&sm.bar_p_full[0], (uint32_t)j & 1u);
-                        tc_gemm_ss_tail(s1_tm, dq1, kd, idS);
-                        tc_commit(&sm.bar_s_full[1]);
-                    }
-                    const uint32_t ks_n = ks + 1 == kKStages ? 0u : ks + 1;
-                    const uint32_t kph_n = ks + 1 == kKStages ? kph ^ 1u : kph;
-                    if (!pv0_ready && !(ok = mbar_wait(&sm.bar_vfull[vs], vph, sm, P.status) &&
-                                             mbar_wait(&sm.bar_p_full[0], (uint32_t)j & 1u, sm, P.status))) break;
-                    tc_fence_after();
-                    const uint64_t vd = dv + vs * kStageDesc;
-                    tc_gemm_ts_head(o0_tm, s0_tm, vd, idO, j > 0 ? 1u : 0u);
-                    k_known = j + 1 < n_tiles && mbar_test(&sm.bar_kfull[ks_n], kph_n);
-                    tc_gemm_ts_tail(o0_tm, s0_tm, vd, idO);
-                    pvs = vs;
-                    if (++vs == kVStages) { vs = 0; vph ^= 1u; }
-                    ks = ks_n;
-                    kph = kph_n;
-                }
-                if (ok) {
-                    tc_commit(&sm.bar_o_done[0]);
-                    if (two && mbar_wait(&sm.bar_p_full[1], (uint32_t)(n_tiles - 1) & 1u, sm, P.status)) {
+                        const uint64_t kd = dk + ks * kStageDesc;
+                        const bool pv1 = two && j > 0;
+                        tc_gemm_ss_head(s0_tm, dq0, kd, idS);
+                        const bool pv1_ready = pv1 && mbar_test(&sm.bar_p_full[1], p1_ph);
+                        tc_gemm_ss_tail(s0_tm, dq0, kd, idS);
+                        tc_commit(&sm.bar_s_full[0]);
+                        if (pv1) {
+                            if (!pv1_ready && !(ok = mbar_wait(&sm.bar_p_full[1], p1_ph, sm, P.status))) break;
+                            tc_fence_after();
+                            const uint64_t vd = dv + pvs * kStageDesc;
+                            tc_gemm_ts_head(o1_tm, s1_tm, vd, idO, j > 1 ? 1u : 0u);
+                            tc_gemm_ts_tail(o1_tm, s1_tm, vd, idO);
+                            p1_ph ^= 1u;
+                        }
+                        bool pv0_ready = false;
+                        if (two) {
+                            tc_gemm_ss_head(s1_tm, dq1, kd, idS);
+                            pv0_ready = mbar_test(&sm.bar_vfull[vs], vph) && mbar_test(&sm.bar_p_full[0], p0_ph);
+                            tc_gemm_ss_tail(s1_tm, dq1, kd, idS);
+                            tc_commit(&sm.bar_s_full[1]);
+                        }
+                        const uint32_t ks_n = ks + 1 == kKStages ? 0u : ks + 1;
+                        const uint32_t kph_n = ks + 1 == kKStages ? kph ^ 1u : kph;
+                        if (!pv0_ready && !(ok = mbar_wait(&sm.bar_vfull[vs], vph, sm, P.status) &&
+                                                 mbar_wait(&sm.bar_p_full[0], p0_ph, sm, P.status))) break;
                         tc_fence_after();
-                        const uint64_t vd = dv + pvs * kStageDesc;
-                        tc_gemm_ts_head(o1_tm, s1_tm, vd, idO, n_tiles > 1 ? 1u : 0u);
-                        tc_gemm_ts_tail(o1_tm, s1_tm, vd, idO);
-                        tc_commit(&sm.bar_o_done[1]);
+                        const uint64_t vd = dv + vs * kStageDesc;
+                        tc_gemm_ts_head(o0_tm, s0_tm, vd, idO, j > 0 ? 1u : 0u);
+                        k_known = j + 1 < n_tiles && mbar_test(&sm.bar_kfull[ks_n], kph_n);
+                        tc_gemm_ts_tail(o0_tm, s0_tm, vd, idO);
+                        p0_ph ^= 1u;
+                        pvs = vs;
+                        if (++vs == kVStages) { vs = 0; vph ^= 1u; }
+                        ks = ks_n;
+                        kph = kph_n;
                     }
+                    if (ok) {
+                        tc_commit(&sm.bar_o_done[0]);
+                        if (two && (ok = mbar_wait(&sm.bar_p_full[1], p1_ph, sm, P.status))) {
+                            tc_fence_after();
+                            const uint64_t vd = dv + pvs * kStageDesc;
+                            tc_gemm_ts_head(o1_tm, s1_tm, vd, idO, n_tiles > 1 ? 1u : 0u);
+                            tc_gemm_ts_tail(o1_tm, s1_tm, vd, idO);
+                            tc_commit(&sm.bar_o_done[1]);
+                            p1_ph ^= 1u;
+                            q1_ph ^= 1u;
+                        }
+                        q0_ph ^= 1u;
+                    }
+                    advance(P, w, n_tiles);
                 }
                 // Drain: every issued MMA lands before TMEM is freed.
                 tc_commit(&sm.bar_mma_done);
@@ -477,203 +496,230 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             }
             __syncwarp();
         }
-            done(P, sm, w);
-        }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
-        for (int turn = 0; sm.left > 0; ++turn) {
         // ========================== softmax + epilogue ========================
         const int qt = (warp - 4) >> 2;
         const int row = (warp & 3) * 32 + lane;        // query row in tile == TMEM lane
-        const Piece w(P, sm);
-        w.set_up(P, sm, turn);
-        const bool any_bad = sm.any_bad[turn & 1];
-        const int h = sm.head, n_tiles = w.n_tiles, r0 = w.u.r0, rows = w.u.rows;
-        const bool active = qt == 0 || w.two;          // this query tile has rows
-        // A row past the last (Q is 0, never stored) takes every key; a warp of
-        // such rows does no softmax.
-        Sees mine = {0, 0};
-        if (active) {
-            // Q: this warp's 32 rows, two rows a pass, 16 lanes on a row's 256 bytes;
-            // rows past the last are zero
-            const int rw = r0 + 128 * qt + (warp & 3) * 32, sub = lane >> 4, chunk = lane & 15;
-            int g = (rw + sub) % P.group;              // row r = i * group + g
-            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(P.attn.q) + w.u.b * P.attn.q_batch_stride +
-                                       (long long)((rw + sub) / P.group) * P.attn.q_row_stride +
-                                       (h * P.group + g) * kKv4Head + 8 * chunk;
-            const long long wrap = P.attn.q_row_stride - P.group * kKv4Head;
-            uint8_t* dst = sm.q[qt] + (chunk >> 3) * kPanel;
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-                const bool in = rw + sub + k < rows;
-                cp_async16(dst + sw128_off((warp & 3) * 32 + sub + k, chunk & 7), in ? src : P.attn.q, in ? 16u : 0u);
-                src += 2 * kKv4Head;
-                for (g += 2; g >= P.group; g -= P.group) src += wrap;
-            }
-            cp_async_wait_all();
-            fence_proxy_async_smem();
-            mbar_arrive(&sm.bar_q[qt]);
-            if (rw + lane < rows) mine = sees(P, w.u.start + (rw + lane) / P.group, w.u.end);
-            else if (rw < rows) mine.hi = 0x7fffffff;
-        }
         const uint32_t s_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u * qt;
         const uint32_t o_tm = s_tm + 256u;
-        float m_run = -INFINITY, l_run = 0.f;          // m in log2 units
+        uint32_t s_ph = 0, o_ph = 0;
         bool ok = true;
-        const int my_tiles = active ? n_tiles : 0;
-        for (int j = 0; j < my_tiles; ++j) {
-            if (!warp_wait(&sm.bar_s_full[qt], (uint32_t)j & 1u, sm, P.status)) { ok = false; break; }
-            tc_fence_after();
-            // S landing for the last query tile of a step means every MMA issued
-            // before has landed: K(j) and V(j-1) are no longer read.
-            if ((int)threadIdx.x == sm.releaser) {
-                mbar_arrive(&sm.bar_kempty[j % kKStages]);
-                if (j > 0) mbar_arrive(&sm.bar_vempty[(j - 1) % kVStages]);
+        // (a wait that ran out ends the list for all four warps at the next turn:
+        // each of them takes part in every sync)
+        for (int turn = 0;; ++turn) {
+            if ((threadIdx.x & 127) == 0) {                // the entry two turns back is read no more
+                Work w = sm.first;
+                if (turn > 0) {
+                    const Turn& was = sm.turn[qt][(turn - 1) & 1];
+                    w = was.w;
+                    advance(P, w, was.n_tiles);
+                }
+                if (w.left > 0 && !*(volatile int*)&sm.abort_flag) {
+                    describe(P, sm.turn[qt][turn & 1], w, sm.first.pos);
+                    if (P.chunked && qt == 0 && w.off == 0) P.ws_unit[1 + w.pair * P.span.kv_heads + w.head] = w.pos;
+                } else {
+                    sm.turn[qt][turn & 1].w.left = 0;
+                }
             }
-            if (__all_sync(0xffffffffu, mine.hi == 0)) {   // no row: what P's columns hold is never stored
+            query_tile_sync(qt);
+            const Turn& pc = sm.turn[qt][turn & 1];
+            if (pc.w.left == 0) break;
+            if (!ok || (qt == 1 && !pc.two)) continue;     // this query tile has no rows
+            const int h = pc.w.head, n_tiles = pc.n_tiles, r0 = pc.row0, rows = pc.rows;
+            const bool releaser = (threadIdx.x & 127) == 0 && qt == pc.two;
+            // A row past the last (Q is 0, never stored) takes every key; a warp of
+            // such rows does no softmax.
+            Sees mine = {0, 0};
+            {
+                // Q: this warp's 32 rows, two rows a pass, 16 lanes on a row's 256 bytes;
+                // rows past the last are zero
+                const int rw = r0 + 128 * qt + (warp & 3) * 32, sub = lane >> 4, chunk = lane & 15;
+                int g = (rw + sub) % P.group;              // row r = i * group + g
+                const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(P.attn.q) +
+                                           pc.batch * P.attn.q_batch_stride +
+                                           (long long)((rw + sub) / P.group) * P.attn.q_row_stride +
+                                           (h * P.group + g) * kKv4Head + 8 * chunk;
+                const long long wrap = P.attn.q_row_stride - P.group * kKv4Head;
+                uint8_t* dst = sm.q[qt] + (chunk >> 3) * kPanel;
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    const bool in = rw + sub + k < rows;
+                    cp_async16(dst + sw128_off((warp & 3) * 32 + sub + k, chunk & 7), in ? src : P.attn.q,
+                               in ? 16u : 0u);
+                    src += 2 * kKv4Head;
+                    for (g += 2; g >= P.group; g -= P.group) src += wrap;
+                }
+                cp_async_wait_all();
+                fence_proxy_async_smem();
+                mbar_arrive(&sm.bar_q[qt]);
+                if (rw + lane < rows) mine = sees(P, pc.start + (rw + lane) / P.group, pc.end);
+                else if (rw < rows) mine.hi = 0x7fffffff;
+            }
+            float m_run = -INFINITY, l_run = 0.f;          // m in log2 units
+            for (int j = 0; j < n_tiles; ++j) {
+                if (!warp_wait(&sm.bar_s_full[qt], s_ph, sm, P.status)) { ok = false; break; }
+                s_ph ^= 1u;
+                tc_fence_after();
+                // (the flag is written before the K tile is full, which S waits for; the
+                // tile that takes its slot cannot begin before this one's P is there)
+                const bool bad = sm.bad[(pc.tile0 + j) % 8];
+                // S landing for the last query tile of a step means every MMA issued
+                // before has landed: K(j) and V(j-1) are no longer read.
+                if (releaser) {
+                    mbar_arrive(&sm.bar_kempty[(pc.tile0 + j) % kKStages]);
+                    if (j > 0) mbar_arrive(&sm.bar_vempty[(pc.tile0 + j - 1) % kVStages]);
+                }
+                if (__all_sync(0xffffffffu, mine.hi == 0)) {   // no row: what P's columns hold is never stored
+                    tc_fence_before();
+                    mbar_arrive(&sm.bar_p_full[qt]);
+                    continue;
+                }
+                uint32_t pk[64];
+                float rsum = 0.f, m_new = m_run;
+                uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                // gone: this row sees no key here
+                bool masked = bad || j >= pc.free_n, gone = false, some_gone = false, all_gone = false;
+                if (masked) {
+                    // columns [0, sink) and [lo, hi) are visible
+                    int u = j + pc.rot;
+                    u = pc.u0 + (u < n_tiles ? u : u - n_tiles);
+                    const int key0 = (u < pc.na ? u : u - pc.na + pc.b0) * kBN;
+                    const int hi = bad ? 0 : mine.hi - key0;
+                    const int sink = P.sink_rows - key0, lo = mine.lo - key0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        vis[e] = below(hi - 32 * e) & (~below(lo - 32 * e) | below(sink - 32 * e));
+                    const uint32_t all = vis[0] & vis[1] & vis[2] & vis[3], any = vis[0] | vis[1] | vis[2] | vis[3];
+                    masked = __any_sync(0xffffffffu, all != any || (any != 0u && all != 0xffffffffu));
+                    // (a warp whose rows each see all or nothing, two frames' rows,
+                    // takes the passes without masks)
+                    gone = any == 0u;
+                    some_gone = __any_sync(0xffffffffu, gone);
+                    all_gone = __all_sync(0xffffffffu, gone);
+                }
+                const bool fresh = m_run == -INFINITY;     // no key seen yet
+                const bool skip = __any_sync(0xffffffffu, fresh && !gone);   // the max first
+                // Exponentials against the running max; rows whose sum overgrows take
+                // the tile's max and do them again.  Where a row sees its first key
+                // the max comes first.
+#pragma unroll 1
+                for (int attempt = skip ? 1 : 0;; ++attempt) {
+                    if ((attempt != 1 || !skip) && !all_gone) {
+                        // (a row without keys keeps max -inf: subtract 0)
+                        const float mm = (m_new == -INFINITY ? 0.f : m_new) - kPShift;
+                        rsum = masked ? exp_visible(s_tm, mm, P.scale_log2, vis, pk)
+                                      : exp_row<false, 4, 0u, true>(s_tm, mm, P.scale_log2, kBN, pk);
+                    }
+                    const bool redo = !gone && (skip ? attempt == 1 : attempt == 0 && !(rsum <= kRedoSum));
+                    if (!__any_sync(0xffffffffu, redo)) break;
+                    const float tmax = masked ? max_visible(s_tm, vis) : max_row<false>(s_tm, kBN);
+                    if (redo) m_new = fmaxf(m_run, tmax * P.scale_log2);
+                }
+                if (some_gone && gone) {
+                    rsum = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) pk[c] = 0u;
+                }
+                const float alpha = m_new == m_run ? 1.f : ex2_approx(m_run - m_new);
+                l_run = l_run * alpha + rsum;
+                m_run = m_new;
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    // O_q holds PV_q(j-1) (complete: it was issued before S_q(j))
+#pragma unroll
+                    for (int c4 = 0; c4 < 4; ++c4) {
+                        uint32_t o[32];
+                        KVP_TMEM_LD32(o_tm + 32 * c4, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                        KVP_TMEM_ST32(o_tm + 32 * c4, o);
+                    }
+                }
+                // P (fp16: off by 2^-11 of itself at most, or 2^-32 of the largest; the
+                // sum keeps 32 bits) -> the first 64 columns of S_q, key 2c in the low half
+                KVP_TMEM_ST32(s_tm, pk);
+                KVP_TMEM_ST32(s_tm + 32, (pk + 32));
+                tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&sm.bar_p_full[qt]);
+            }
+            // A warp's rows go out through its own rows of the Q tile (every S
+            // has landed): a row's 128 bytes by eight lanes, four rows a store.
+            const int er = pc.rows, r = pc.row0 + 128 * qt + row;
+            const bool partial = pc.partial;
+            if (!ok || !warp_wait(&sm.bar_o_done[qt], o_ph, sm, P.status)) {
+                ok = false;
                 continue;
             }
-            uint32_t pk[64];
-            float rsum = 0.f, m_new = m_run;
-            uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-            // gone: this row sees no key here
-            bool masked = any_bad || j >= sm.free_n, gone = false, some_gone = false, all_gone = false;
-            if (masked) {
-                // columns [0, sink) and [lo, hi) are visible
-                int u = j + sm.rot;
-                u = sm.u0 + (u < sm.n_tiles ? u : u - sm.n_tiles);
-                const int pos = u < sm.na ? u : u - sm.na + sm.b0, key0 = pos * kBN;
-                int hi = mine.hi - key0;
-                if (any_bad && page_of(s, sm.batch, pos) < 0) hi = 0;
-                const int sink = P.sink_rows - key0, lo = mine.lo - key0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    vis[e] = below(hi - 32 * e) & (~below(lo - 32 * e) | below(sink - 32 * e));
-                masked = __any_sync(0xffffffffu, (vis[0] & vis[1] & vis[2] & vis[3]) != (vis[0] | vis[1] | vis[2] | vis[3]) ||
-                                                     vis[0] + 1u > 1u);
-                // (a warp whose rows each see all or nothing, two frames' rows,
-                // takes the passes without masks)
-                gone = (vis[0] | vis[1] | vis[2] | vis[3]) == 0u;
-                some_gone = __any_sync(0xffffffffu, gone);
-                all_gone = __all_sync(0xffffffffu, gone);
-            }
-            const bool fresh = m_run == -INFINITY;     // no key seen yet
-            const bool skip = __any_sync(0xffffffffu, fresh && !gone);   // the max first
-            // Exponentials against the running max; rows whose sum overgrows take
-            // the tile's max and do them again.  Where a row sees its first key
-            // the max comes first.
+            o_ph ^= 1u;
+            tc_fence_after();
+            if (releaser) mbar_arrive(&sm.bar_vempty[(pc.tile0 + n_tiles - 1) % kVStages]);
+            uint8_t* stage = sm.q[qt] + (warp & 3) * 32 * 128;
+            const int rw = r - lane, sub = lane >> 3, chunk = lane & 7;
+            const float inv = l_run == 0.f ? 0.f : kVUnit / l_run;      // a row without keys is 0
+            // row rw + sub + 4 i of the workspace or of the output
+            const long long slot = unit_slot((int)blockIdx.x, pc.u0 == 0) * 256 + 128 * qt + (warp & 3) * 32;
+            if (partial)
+                *reinterpret_cast<float2*>(P.ws_ml + (slot + lane) * 2) = make_float2(m_run, l_run);
+            uint8_t* ws = reinterpret_cast<uint8_t*>(P.ws_o + (slot + sub) * kKv4Head) + 16 * chunk;
+            uint8_t* out = reinterpret_cast<uint8_t*>(static_cast<__nv_bfloat16*>(P.attn.out) +
+                                                      pc.batch * P.attn.out_batch_stride +
+                                                      (long long)h * P.group * kKv4Head) + 16 * chunk;
+            const int step = partial ? 32 : 64;                         // dims that make 128 bytes
 #pragma unroll 1
-            for (int attempt = skip ? 1 : 0;; ++attempt) {
-                if ((attempt != 1 || !skip) && !all_gone) {
-                    // (a row without keys keeps max -inf: subtract 0)
-                    const float mm = (m_new == -INFINITY ? 0.f : m_new) - kPShift;
-                    rsum = masked ? exp_visible(s_tm, mm, P.scale_log2, vis, pk)
-                                  : exp_row<false, 4, 0u, true>(s_tm, mm, P.scale_log2, kBN, pk);
-                }
-                const bool redo = !gone && (skip ? attempt == 1 : attempt == 0 && !(rsum <= kRedoSum));
-                if (!__any_sync(0xffffffffu, redo)) break;
-                const float tmax = masked ? max_visible(s_tm, vis) : max_row<false>(s_tm, kBN);
-                if (redo) m_new = fmaxf(m_run, tmax * P.scale_log2);
-            }
-            if (some_gone && gone) {
-                rsum = 0.f;
+            for (int c0 = 0; c0 < kKv4Head; c0 += step) {
+                uint32_t o[32];
+                KVP_TMEM_LD32(o_tm + c0, o);
+                KVP_TMEM_WAIT_LD_DEP(o);
+                if (partial) {
 #pragma unroll
-                for (int c = 0; c < 64; ++c) pk[c] = 0u;
-            }
-            const float alpha = m_new == m_run ? 1.f : ex2_approx(m_run - m_new);
-            l_run = l_run * alpha + rsum;
-            m_run = m_new;
-            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                // O_q holds PV_q(j-1) (complete: it was issued before S_q(j))
-#pragma unroll
-                for (int c4 = 0; c4 < 4; ++c4) {
-                    uint32_t o[32];
-                    KVP_TMEM_LD32(o_tm + 32 * c4, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-                    KVP_TMEM_ST32(o_tm + 32 * c4, o);
-                }
-            }
-            // P (fp16: off by 2^-11 of itself at most, or 2^-32 of the largest; the
-            // sum keeps 32 bits) -> the first 64 columns of S_q, key 2c in the low half
-            KVP_TMEM_ST32(s_tm, pk);
-            KVP_TMEM_ST32(s_tm + 32, (pk + 32));
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&sm.bar_p_full[qt]);
-        }
-        // A warp's rows go out through its own rows of the Q tile (every S
-        // has landed): a row's 128 bytes by eight lanes, four rows a store.
-        const int er = sm.rows, r = sm.row0 + 128 * qt + row;
-        const bool partial = sm.partial;
-        if (ok && my_tiles > 0) ok = warp_wait(&sm.bar_o_done[qt], 0, sm, P.status);
-        tc_fence_after();
-        uint8_t* stage = sm.q[qt] + (warp & 3) * 32 * 128;
-        const int rw = r - lane, sub = lane >> 3, chunk = lane & 7;
-        const float inv = l_run == 0.f ? 0.f : kVUnit / l_run;      // a row without keys is 0
-        // row rw + sub + 4 i of the workspace or of the output
-        const long long slot = unit_slot((int)blockIdx.x, sm.u0 == 0) * 256 + 128 * qt + (warp & 3) * 32;
-        if (partial && ok && active)
-            *reinterpret_cast<float2*>(P.ws_ml + (slot + lane) * 2) = make_float2(m_run, l_run);
-        uint8_t* ws = reinterpret_cast<uint8_t*>(P.ws_o + (slot + sub) * kKv4Head) + 16 * chunk;
-        uint8_t* out = reinterpret_cast<uint8_t*>(static_cast<__nv_bfloat16*>(P.attn.out) +
-                                                  sm.batch * P.attn.out_batch_stride +
-                                                  (long long)sm.head * P.group * kKv4Head) + 16 * chunk;
-        const int step = partial ? 32 : 64;                         // dims that make 128 bytes
+                    for (int c = 0; c < 8; ++c)
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                            make_uint4(__float_as_uint(__uint_as_float(o[4 * c]) * kVUnit),
+                                       __float_as_uint(__uint_as_float(o[4 * c + 1]) * kVUnit),
+                                       __float_as_uint(__uint_as_float(o[4 * c + 2]) * kVUnit),
+                                       __float_as_uint(__uint_as_float(o[4 * c + 3]) * kVUnit));
+                } else {
 #pragma unroll 1
-        for (int c0 = 0; ok && my_tiles > 0 && c0 < kKv4Head; c0 += step) {
-            uint32_t o[32];
-            KVP_TMEM_LD32(o_tm + c0, o);
-            KVP_TMEM_WAIT_LD_DEP(o);
-            if (partial) {
+                    for (int e = 0; e < 2; ++e) {
+                        if (e) {
+                            KVP_TMEM_LD32(o_tm + c0 + 32, o);
+                            KVP_TMEM_WAIT_LD_DEP(o);
+                        }
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                        make_uint4(__float_as_uint(__uint_as_float(o[4 * c]) * kVUnit),
-                                   __float_as_uint(__uint_as_float(o[4 * c + 1]) * kVUnit),
-                                   __float_as_uint(__uint_as_float(o[4 * c + 2]) * kVUnit),
-                                   __float_as_uint(__uint_as_float(o[4 * c + 3]) * kVUnit));
-            } else {
-#pragma unroll 1
-                for (int e = 0; e < 2; ++e) {
-                    if (e) {
-                        KVP_TMEM_LD32(o_tm + c0 + 32, o);
-                        KVP_TMEM_WAIT_LD_DEP(o);
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint4 y;
-                        y.x = pack_bf16(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv);
-                        y.y = pack_bf16(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv);
-                        y.z = pack_bf16(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv);
-                        y.w = pack_bf16(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv);
-                        *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * e + c) ^ (lane & 7)) << 4)) = y;
+                        for (int c = 0; c < 4; ++c) {
+                            uint4 y;
+                            y.x = pack_bf16(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv);
+                            y.y = pack_bf16(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv);
+                            y.z = pack_bf16(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv);
+                            y.w = pack_bf16(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv);
+                            *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * e + c) ^ (lane & 7)) << 4)) = y;
+                        }
                     }
                 }
-            }
-            __syncwarp();
-            int qi = (rw + sub) / P.group, qg = (rw + sub) % P.group;   // row = qi * group + qg
+                __syncwarp();
+                int qi = (rw + sub) / P.group, qg = (rw + sub) % P.group;   // row = qi * group + qg
 #pragma unroll 4
-            for (int i = 0; i < 8; ++i) {
-                const int k = 4 * i + sub;
-                const uint4 y = *reinterpret_cast<const uint4*>(stage + k * 128 + ((chunk ^ (k & 7)) << 4));
-                uint8_t* dst = partial ? ws + i * (4 * kKv4Head * 4) + c0 * 4
-                                       : out + (qi * P.attn.out_row_stride + qg * kKv4Head + c0) * 2;
-                if (rw + k < er) *reinterpret_cast<uint4*>(dst) = y;
-                if (!partial)
-                    for (qg += 4; qg >= P.group; qg -= P.group) ++qi;
+                for (int i = 0; i < 8; ++i) {
+                    const int k = 4 * i + sub;
+                    const uint4 y = *reinterpret_cast<const uint4*>(stage + k * 128 + ((chunk ^ (k & 7)) << 4));
+                    uint8_t* dst = partial ? ws + i * (4 * kKv4Head * 4) + c0 * 4
+                                           : out + (qi * P.attn.out_row_stride + qg * kKv4Head + c0) * 2;
+                    if (rw + k < er) *reinterpret_cast<uint4*>(dst) = y;
+                    if (!partial)
+                        for (qg += 4; qg >= P.group; qg -= P.group) ++qi;
+                }
+                __syncwarp();
             }
-            __syncwarp();
-        }
-            done(P, sm, w);
+            tc_fence_before();                             // O is read: the next piece may begin to fill it
         }
     }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
     if (warp == 1) {
-        tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }

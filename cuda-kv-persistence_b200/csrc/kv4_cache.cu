@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const Kv4Span s, T* 
                 e[0][i] = it.blk[kKv4KScale + r * 8 + (word >> 1)];
             }
             if (v) {
-                c[1][i] = *reinterpret_cast<const uint32_t*>(it.blk + kKv4VCode + (word >> 1) * 64 + r * 8 + (word & 1) * 4);
+                c[1][i] = *reinterpret_cast<const uint32_t*>(it.blk + kKv4VCode + (word >> 1) * 64 + r * 8 +
+                                                             (word & 1) * 4);
                 e[1][i] = it.blk[kKv4VScale + (word >> 1) * 8 + r];
             }
         }
