@@ -91,7 +91,7 @@ struct __align__(1024) Smem {
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // 128 columns of an S row of which vis says which are visible (32 a word; a
-// warp's rows agree on most words) -> P, their sum; and their max.  A hidden
+// warp's rows agree on most words): their max, and P with its sum.  A hidden
 // key's weight is 0: everything on MUFU, whose 2^-inf is 0.
 __device__ __forceinline__ void load_visible(uint32_t s_addr, uint32_t vis, uint32_t (&y)[32]) {
     KVP_TMEM_LD32(s_addr, y);
@@ -101,6 +101,19 @@ __device__ __forceinline__ void load_visible(uint32_t s_addr, uint32_t vis, uint
         for (int c = 0; c < 32; ++c)
             if (!(vis >> c & 1u)) y[c] = 0xFF800000u;   // -inf
     }
+}
+__device__ __forceinline__ float max_visible(uint32_t s_addr, const uint32_t (&vis)[4]) {
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+    for (int h = 0; h < 4; ++h) {
+        const uint32_t v = h == 0 ? vis[0] : h == 1 ? vis[1] : h == 2 ? vis[2] : vis[3];
+        if (__all_sync(0xffffffffu, v == 0u)) continue;
+        uint32_t y[32];
+        load_visible(s_addr + 32 * h, v, y);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(y[c]));
+    }
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 __device__ __forceinline__ float exp_visible(uint32_t s_addr, float m, float sl2, const uint32_t (&vis)[4],
                                              uint32_t (&pk)[64]) {
@@ -126,21 +139,6 @@ __device__ __forceinline__ float exp_visible(uint32_t s_addr, float m, float sl2
         sum += part[0] + part[1];
     }
     return sum;
-}
-__device__ __forceinline__ float max_visible(uint32_t s_addr, const uint32_t (&vis)[4]) {
-    float m = -INFINITY;
-#pragma unroll 1
-    for (int h = 0; h < 4; ++h) {
-        const uint32_t v = h == 0 ? vis[0] : h == 1 ? vis[1] : h == 2 ? vis[2] : vis[3];
-        if (__all_sync(0xffffffffu, v == 0u)) continue;
-        uint32_t y[32];
-        load_visible(s_addr + 32 * h, v, y);
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(y[c]));
-        m = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-    }
-    return m;
 }
 
 // A word's eight values, K in bf16 and V in fp16, and a lane's four words as
@@ -557,30 +555,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 else if (rw < rows) mine.hi = 0x7fffffff;
             }
             float m_run = -INFINITY, l_run = 0.f;          // m in log2 units
+            bool warm = false;                             // every row of the warp has seen a key
+            const int free_n = pc.free_n, tile0 = pc.tile0;
             for (int j = 0; j < n_tiles; ++j) {
                 if (!warp_wait(&sm.bar_s_full[qt], s_ph, sm, P.status)) { ok = false; break; }
                 s_ph ^= 1u;
                 tc_fence_after();
                 // (the flag is written before the K tile is full, which S waits for; the
                 // tile that takes its slot cannot begin before this one's P is there)
-                const bool bad = sm.bad[(pc.tile0 + j) % 8];
+                const bool bad = sm.bad[(tile0 + j) % 8];
                 // S landing for the last query tile of a step means every MMA issued
                 // before has landed: K(j) and V(j-1) are no longer read.
                 if (releaser) {
-                    mbar_arrive(&sm.bar_kempty[(pc.tile0 + j) % kKStages]);
-                    if (j > 0) mbar_arrive(&sm.bar_vempty[(pc.tile0 + j - 1) % kVStages]);
+                    mbar_arrive(&sm.bar_kempty[(tile0 + j) % kKStages]);
+                    if (j > 0) mbar_arrive(&sm.bar_vempty[(tile0 + j - 1) % kVStages]);
                 }
                 if (__all_sync(0xffffffffu, mine.hi == 0)) {   // no row: what P's columns hold is never stored
                     tc_fence_before();
                     mbar_arrive(&sm.bar_p_full[qt]);
                     continue;
                 }
-                uint32_t pk[64];
-                float rsum = 0.f, m_new = m_run;
                 uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-                // gone: this row sees no key here
-                bool masked = bad || j >= pc.free_n, gone = false, some_gone = false, all_gone = false;
-                if (masked) {
+                bool gone = false, some_gone = false;      // (a row that sees nothing here)
+                bool plain = warm;                         // each row sees all or nothing, and has a max
+                if (__builtin_expect(bad || j >= free_n, 0)) {
                     // columns [0, sink) and [lo, hi) are visible
                     int u = j + pc.rot;
                     u = pc.u0 + (u < n_tiles ? u : u - n_tiles);
@@ -590,55 +588,66 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         vis[e] = below(hi - 32 * e) & (~below(lo - 32 * e) | below(sink - 32 * e));
-                    const uint32_t all = vis[0] & vis[1] & vis[2] & vis[3], any = vis[0] | vis[1] | vis[2] | vis[3];
-                    masked = __any_sync(0xffffffffu, all != any || (any != 0u && all != 0xffffffffu));
-                    // (a warp whose rows each see all or nothing, two frames' rows,
-                    // takes the passes without masks)
-                    gone = any == 0u;
+                    const bool whole = (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu;
+                    gone = (vis[0] | vis[1] | vis[2] | vis[3]) == 0u;
                     some_gone = __any_sync(0xffffffffu, gone);
-                    all_gone = __all_sync(0xffffffffu, gone);
+                    plain = __all_sync(0xffffffffu, gone || (whole && m_run != -INFINITY)) &&
+                            !__all_sync(0xffffffffu, gone);
                 }
-                const bool fresh = m_run == -INFINITY;     // no key seen yet
-                const bool skip = __any_sync(0xffffffffu, fresh && !gone);   // the max first
-                // Exponentials against the running max; rows whose sum overgrows take
-                // the tile's max and do them again.  Where a row sees its first key
-                // the max comes first.
+                // P (fp16: off by 2^-11 of itself at most, or 2^-32 of the largest;
+                // the sum keeps 32 bits) -> the first 64 columns of S_q, key 2c in
+                // the low half.  Nearly every tile goes the first way, against the
+                // running max, which is laid out without a jump (700 cycles stood
+                // between S and the first exponential before).
+                uint32_t pk[64];
+                float rsum = 0.f;
+                bool done = plain;
+                if (__builtin_expect(plain, 1)) {
+                    rsum = exp_row<false, 4, 0u, true>(s_tm, m_run - kPShift, P.scale_log2, kBN, pk);
+                    if (__builtin_expect(some_gone, 0)) {
+                        if (gone) {
+                            rsum = 0.f;
+#pragma unroll
+                            for (int c = 0; c < 64; ++c) pk[c] = 0u;
+                        }
+                    }
+                    done = __all_sync(0xffffffffu, rsum <= kRedoSum);
+                }
+                if (__builtin_expect(!done, 0)) {
+                    // Hidden keys, a row's first key (the max comes first then) or a
+                    // row whose sum overgrows (it takes the tile's max and goes again).
+                    const bool first = __any_sync(0xffffffffu, m_run == -INFINITY && !gone);
+                    float m_new = m_run;
 #pragma unroll 1
-                for (int attempt = skip ? 1 : 0;; ++attempt) {
-                    if ((attempt != 1 || !skip) && !all_gone) {
+                    for (int pass = first || plain ? 1 : 0; pass < 2; ++pass) {
+                        if (pass == 1) {
+                            const bool raise = !gone && (first || !(rsum <= kRedoSum));
+                            if (!__any_sync(0xffffffffu, raise)) break;
+                            const float top = max_visible(s_tm, vis);
+                            if (raise) m_new = fmaxf(m_run, top * P.scale_log2);
+                        }
                         // (a row without keys keeps max -inf: subtract 0)
-                        const float mm = (m_new == -INFINITY ? 0.f : m_new) - kPShift;
-                        rsum = masked ? exp_visible(s_tm, mm, P.scale_log2, vis, pk)
-                                      : exp_row<false, 4, 0u, true>(s_tm, mm, P.scale_log2, kBN, pk);
+                        rsum = exp_visible(s_tm, (m_new == -INFINITY ? 0.f : m_new) - kPShift, P.scale_log2, vis, pk);
                     }
-                    const bool redo = !gone && (skip ? attempt == 1 : attempt == 0 && !(rsum <= kRedoSum));
-                    if (!__any_sync(0xffffffffu, redo)) break;
-                    const float tmax = masked ? max_visible(s_tm, vis) : max_row<false>(s_tm, kBN);
-                    if (redo) m_new = fmaxf(m_run, tmax * P.scale_log2);
-                }
-                if (some_gone && gone) {
-                    rsum = 0.f;
+                    const float alpha = m_new == m_run ? 1.f : ex2_approx(m_run - m_new);
+                    l_run *= alpha;
+                    m_run = m_new;
+                    warm = __all_sync(0xffffffffu, m_run != -INFINITY);
+                    if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                        // O_q holds PV_q(j-1) (complete: it was issued before S_q(j))
+#pragma unroll 1
+                        for (int c4 = 0; c4 < 4; ++c4) {
+                            uint32_t o[32];
+                            KVP_TMEM_LD32(o_tm + 32 * c4, o);
+                            KVP_TMEM_WAIT_LD_DEP(o);
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) pk[c] = 0u;
-                }
-                const float alpha = m_new == m_run ? 1.f : ex2_approx(m_run - m_new);
-                l_run = l_run * alpha + rsum;
-                m_run = m_new;
-                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                    // O_q holds PV_q(j-1) (complete: it was issued before S_q(j))
-#pragma unroll
-                    for (int c4 = 0; c4 < 4; ++c4) {
-                        uint32_t o[32];
-                        KVP_TMEM_LD32(o_tm + 32 * c4, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-                        KVP_TMEM_ST32(o_tm + 32 * c4, o);
+                            for (int c = 0; c < 32; ++c)
+                                o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                            KVP_TMEM_ST32(o_tm + 32 * c4, o);
+                        }
                     }
                 }
-                // P (fp16: off by 2^-11 of itself at most, or 2^-32 of the largest; the
-                // sum keeps 32 bits) -> the first 64 columns of S_q, key 2c in the low half
+                l_run += rsum;
                 KVP_TMEM_ST32(s_tm, pk);
                 KVP_TMEM_ST32(s_tm + 32, (pk + 32));
                 tmem_wait_st();
@@ -655,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             }
             o_ph ^= 1u;
             tc_fence_after();
-            if (releaser) mbar_arrive(&sm.bar_vempty[(pc.tile0 + n_tiles - 1) % kVStages]);
+            if (releaser) mbar_arrive(&sm.bar_vempty[(tile0 + n_tiles - 1) % kVStages]);
             uint8_t* stage = sm.q[qt] + (warp & 3) * 32 * 128;
             const int rw = r - lane, sub = lane >> 3, chunk = lane & 7;
             const float inv = l_run == 0.f ? 0.f : kVUnit / l_run;      // a row without keys is 0
