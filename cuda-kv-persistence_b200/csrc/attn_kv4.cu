@@ -585,6 +585,7 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     P.sink_rows = (int)std::min<long long>((long long)a.sinks * a.tokens, cap);
     P.scale_log2 = 1.4426950408889634f / sqrtf((float)kKv4Head);
     P.rise = kRise / P.scale_log2;
+    P.inv_group = 1.f / (float)P.group;
 
     // Keys that the rows of one tile can see, at most (starts on the device: the
     // capacity's).

@@ -24,6 +24,7 @@ struct Kv4Params {
     int chunked;             // (many rows) the CTAs share the list of all units' pages evenly: see Kv4Unit
     float scale_log2;        // log2(e) / sqrt(128)
     float rise;              // kRise in score units
+    float inv_group;         // 1 / group
 };
 
 namespace kv4_dev {

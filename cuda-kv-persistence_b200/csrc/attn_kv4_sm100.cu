@@ -62,11 +62,14 @@ struct Work {
     int pair, head, off, left, pos;
 };
 
-// A piece for the softmax, which holds little of it in registers.
+// A piece for the softmax, which holds little of it in registers.  An expander,
+// which is ahead, makes the entries (a piece's dozen divisions are 1,400 cycles
+// that would stand between two pieces).
 struct Turn {
-    Work w;
-    volatile int batch, start, end, rows, row0, u0, n_tiles, rot, na, b0, two, partial, free_n, tile0;
+    int batch, head, start, end, rows, row0, u0, n_tiles, rot, na, b0, two, partial, free_n, tile0;
+    int qi0, qg0;               // row row0 is query head qg0 of the group, of the sequence's row qi0
 };
+constexpr int kTurns = 4;
 
 struct __align__(1024) Smem {
     uint8_t q[2][kTileBytes];
@@ -78,13 +81,14 @@ struct __align__(1024) Smem {
     uint64_t bar_s_full[2];     // S_q(j) landed (and, by issue order, PV_q(j-1) too)
     uint64_t bar_p_full[2];     // P_q(j) in TMEM, S_q(j) read, O_q rescaled
     uint64_t bar_o_done[2];     // last PV_q landed
+    uint64_t bar_turn[kTurns], bar_turn_empty[kTurns];
     uint64_t bar_mma_done;      // every issued MMA landed (TMEM may be freed)
     uint32_t tmem_base;
     int abort_flag;
     int scan[kThreads / 32];
     Work first;                 // where the CTA begins
     volatile int bad[8];        // K/V tile i of the CTA: its page is not in the pool (slot i % 8)
-    Turn turn[2][2];            // [query tile][piece % 2]
+    Turn turn[kTurns];          // piece i: slot i % kTurns; n_tiles 0 ends the list
 };
 
 // Bits [0, n) set.
@@ -175,6 +179,10 @@ __device__ __forceinline__ void init_barriers(Smem& sm) {
         mbar_init(&sm.bar_vfull[i], kUnits / 2);
         mbar_init(&sm.bar_vempty[i], 1);
     }
+    for (int i = 0; i < kTurns; ++i) {
+        mbar_init(&sm.bar_turn[i], 1);
+        mbar_init(&sm.bar_turn_empty[i], 8);
+    }
     mbar_init(&sm.bar_mma_done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -218,29 +226,16 @@ __device__ __forceinline__ void advance(const Kv4Params& P, Work& w, int n_tiles
     }
 }
 
-// A piece's entry for the softmax (tile0: the CTA's K/V tiles before it).
-__device__ __forceinline__ void describe(const Kv4Params& P, Turn& t, const Work& w, int first_pos) {
-    const Piece p(P, w);
-    t.w = w;
-    t.batch = p.u.b;
-    t.start = p.u.start;
-    t.end = p.u.end;
-    t.rows = p.u.rows;
-    t.row0 = p.u.r0;
-    t.u0 = p.u0;
-    t.n_tiles = p.n_tiles;
-    t.rot = p.rot;
-    t.na = p.u.na;
-    t.b0 = p.u.b0;
-    t.two = p.two;
-    t.partial = p.n_tiles < p.u.pages;
-    t.free_n = max(p.free1() - p.free0(), 0);
-    t.tile0 = w.pos - first_pos;
-}
-
-__device__ __forceinline__ void query_tile_sync(int qt) {     // its four warps
-    if (qt) asm volatile("bar.sync 2, 128;" ::: "memory");
-    else asm volatile("bar.sync 1, 128;" ::: "memory");
+// Row row0 + i (i < 256) of a piece: query head g of the group, the sequence's
+// row.  (t + 1/2) / group is 2^-9 from an integer at least where group is below
+// 256, far from fp32's rounding; above it the quotient is 0 or 1.
+struct RowOf {
+    int row, g;
+};
+__device__ __forceinline__ RowOf row_of(const Kv4Params& P, int qi0, int qg0, int i) {
+    const int t = qg0 + i;
+    const int q = P.group < 256 ? (int)(((float)t + 0.5f) * P.inv_group) : t >= P.group ? 1 : 0;
+    return RowOf{qi0 + q, t - q * P.group};
 }
 
 __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __grid_constant__ Kv4Params P) {
@@ -335,9 +330,39 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             }
             const uint32_t page_bytes = (uint32_t)s.kv_heads * kKv4PageHeadBytes;
             const int turn0 = warp == 0 ? 0 : warp - 1;    // its first unit of a piece
+            // slot `turn` is free: the eight softmax warps are done with the piece before
+            auto next_turn = [&](int turn) {
+                return warp_wait(&sm.bar_turn_empty[turn % kTurns], (uint32_t)(turn / kTurns & 1) ^ 1u, sm, P.status);
+            };
             bool ok = true;
+            int turn = 0;
             for (int tile0 = 0; ok && w.left > 0;) {
                 const Piece pc(P, w);
+                if (warp == 0) ok = next_turn(turn);
+                if (!ok) break;
+                if (warp == 0 && lane == 0) {
+                    Turn& t = sm.turn[turn % kTurns];
+                    t.batch = pc.u.b;
+                    t.head = w.head;
+                    t.start = pc.u.start;
+                    t.end = pc.u.end;
+                    t.rows = pc.u.rows;
+                    t.row0 = pc.u.r0;
+                    t.u0 = pc.u0;
+                    t.n_tiles = pc.n_tiles;
+                    t.rot = pc.rot;
+                    t.na = pc.u.na;
+                    t.b0 = pc.u.b0;
+                    t.two = pc.two;
+                    t.partial = pc.n_tiles < pc.u.pages;
+                    t.free_n = max(pc.free1() - pc.free0(), 0);
+                    t.tile0 = tile0;
+                    t.qi0 = pc.u.r0 / P.group;
+                    t.qg0 = pc.u.r0 % P.group;
+                    if (P.chunked && w.off == 0) P.ws_unit[1 + w.pair * s.kv_heads + w.head] = w.pos;
+                    mbar_arrive(&sm.bar_turn[turn % kTurns]);
+                }
+                ++turn;
                 const int units = pc.n_tiles * kUnits;
                 const uint8_t* pool = static_cast<const uint8_t*>(s.pages) + w.head * kKv4PageHeadBytes;
                 auto lookup = [&](int n) { return n < units ? page_of(s, pc.u.b, pc.page_pos(n / kUnits)) : 0; };
@@ -408,6 +433,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 }
                 tile0 += pc.n_tiles;
                 advance(P, w, pc.n_tiles);
+            }
+            if (warp == 0 && ok && next_turn(turn) && lane == 0) {
+                sm.turn[turn % kTurns].n_tiles = 0;
+                mbar_arrive(&sm.bar_turn[turn % kTurns]);
             }
         } else {
             // ============================ MMA issuer ==========================
@@ -503,28 +532,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
         const uint32_t o_tm = s_tm + 256u;
         uint32_t s_ph = 0, o_ph = 0;
         bool ok = true;
-        // (a wait that ran out ends the list for all four warps at the next turn:
-        // each of them takes part in every sync)
-        for (int turn = 0;; ++turn) {
-            if ((threadIdx.x & 127) == 0) {                // the entry two turns back is read no more
-                Work w = sm.first;
-                if (turn > 0) {
-                    const Turn& was = sm.turn[qt][(turn - 1) & 1];
-                    w = was.w;
-                    advance(P, w, was.n_tiles);
-                }
-                if (w.left > 0 && !*(volatile int*)&sm.abort_flag) {
-                    describe(P, sm.turn[qt][turn & 1], w, sm.first.pos);
-                    if (P.chunked && qt == 0 && w.off == 0) P.ws_unit[1 + w.pair * P.span.kv_heads + w.head] = w.pos;
-                } else {
-                    sm.turn[qt][turn & 1].w.left = 0;
-                }
+        for (int turn = 0; ok; ++turn) {
+            if (!warp_wait(&sm.bar_turn[turn % kTurns], (uint32_t)(turn / kTurns) & 1u, sm, P.status)) break;
+            const volatile Turn& pc = sm.turn[turn % kTurns];
+            const int n_tiles = pc.n_tiles;
+            if (n_tiles == 0) break;
+            if (qt == 1 && !pc.two) {                      // this query tile has no rows
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.bar_turn_empty[turn % kTurns]);
+                continue;
             }
-            query_tile_sync(qt);
-            const Turn& pc = sm.turn[qt][turn & 1];
-            if (pc.w.left == 0) break;
-            if (!ok || (qt == 1 && !pc.two)) continue;     // this query tile has no rows
-            const int h = pc.w.head, n_tiles = pc.n_tiles, r0 = pc.row0, rows = pc.rows;
+            const int h = pc.head, r0 = pc.row0, rows = pc.rows, qi0 = pc.qi0, qg0 = pc.qg0;
             const bool releaser = (threadIdx.x & 127) == 0 && qt == pc.two;
             // A row past the last (Q is 0, never stored) takes every key; a warp of
             // such rows does no softmax.
@@ -532,26 +550,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             {
                 // Q: this warp's 32 rows, two rows a pass, 16 lanes on a row's 256 bytes;
                 // rows past the last are zero
-                const int rw = r0 + 128 * qt + (warp & 3) * 32, sub = lane >> 4, chunk = lane & 15;
-                int g = (rw + sub) % P.group;              // row r = i * group + g
+                const int mine0 = 128 * qt + (warp & 3) * 32, rw = r0 + mine0, sub = lane >> 4, chunk = lane & 15;
                 const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(P.attn.q) +
                                            pc.batch * P.attn.q_batch_stride +
-                                           (long long)((rw + sub) / P.group) * P.attn.q_row_stride +
-                                           (h * P.group + g) * kKv4Head + 8 * chunk;
-                const long long wrap = P.attn.q_row_stride - P.group * kKv4Head;
+                                           (long long)h * P.group * kKv4Head + 8 * chunk;
                 uint8_t* dst = sm.q[qt] + (chunk >> 3) * kPanel;
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
                     const bool in = rw + sub + k < rows;
-                    cp_async16(dst + sw128_off((warp & 3) * 32 + sub + k, chunk & 7), in ? src : P.attn.q,
-                               in ? 16u : 0u);
-                    src += 2 * kKv4Head;
-                    for (g += 2; g >= P.group; g -= P.group) src += wrap;
+                    const RowOf y = row_of(P, qi0, qg0, mine0 + sub + k);
+                    cp_async16(dst + sw128_off((warp & 3) * 32 + sub + k, chunk & 7),
+                               in ? src + y.row * P.attn.q_row_stride + (long long)y.g * kKv4Head : P.attn.q, in ? 16u : 0u);
                 }
                 cp_async_wait_all();
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.bar_q[qt]);
-                if (rw + lane < rows) mine = sees(P, pc.start + (rw + lane) / P.group, pc.end);
+                if (rw + lane < rows) mine = sees(P, pc.start + row_of(P, qi0, qg0, mine0 + lane).row, pc.end);
                 else if (rw < rows) mine.hi = 0x7fffffff;
             }
             float m_run = -INFINITY, l_run = 0.f;          // m in log2 units
@@ -660,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             const bool partial = pc.partial;
             if (!ok || !warp_wait(&sm.bar_o_done[qt], o_ph, sm, P.status)) {
                 ok = false;
-                continue;
+                break;
             }
             o_ph ^= 1u;
             tc_fence_after();
@@ -709,20 +723,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                     }
                 }
                 __syncwarp();
-                int qi = (rw + sub) / P.group, qg = (rw + sub) % P.group;   // row = qi * group + qg
 #pragma unroll 4
                 for (int i = 0; i < 8; ++i) {
                     const int k = 4 * i + sub;
                     const uint4 y = *reinterpret_cast<const uint4*>(stage + k * 128 + ((chunk ^ (k & 7)) << 4));
-                    uint8_t* dst = partial ? ws + i * (4 * kKv4Head * 4) + c0 * 4
-                                           : out + (qi * P.attn.out_row_stride + qg * kKv4Head + c0) * 2;
+                    uint8_t* dst = ws + i * (4 * kKv4Head * 4) + c0 * 4;
+                    if (!partial) {
+                        const RowOf x = row_of(P, qi0, qg0, 128 * qt + (warp & 3) * 32 + k);
+                        dst = out + (x.row * P.attn.out_row_stride + (long long)x.g * kKv4Head + c0) * 2;
+                    }
                     if (rw + k < er) *reinterpret_cast<uint4*>(dst) = y;
-                    if (!partial)
-                        for (qg += 4; qg >= P.group; qg -= P.group) ++qi;
                 }
                 __syncwarp();
             }
             tc_fence_before();                             // O is read: the next piece may begin to fill it
+            if (lane == 0) mbar_arrive(&sm.bar_turn_empty[turn % kTurns]);
         }
     }
     tc_fence_before();
