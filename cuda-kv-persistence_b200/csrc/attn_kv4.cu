@@ -597,9 +597,9 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     // Up to 16 rows of a K/V head fit the N side of the mma.sync kernel; more go
     // through it 16 at a time as long as that is quicker.  It takes a thousand
     // 16-row x 32-key steps in 1.5 us after 7 us, the tcgen05 kernel a thousand
-    // of 256 rows in 4.1 us after 17 (12 heads x 4064 keys, 64 rows: 17.8 us and
-    // 25.0; 2 x 8 heads x 9064 keys, 32 rows: 19.1 and 41.2, 64 rows: 31.1 and
-    // 42.1; 16 x 8 heads x 8064 keys, 32 rows: 96.5 and 154, 64 rows: 190 and 153).
+    // of 256 rows in 4.1 us after 17 (12 heads x 4064 keys, 64 rows: 17.7 us and
+    // 27.2; 2 x 8 heads x 9064 keys, 32 rows: 19.3 and 37.0, 64 rows: 31.5 and
+    // 38.5; 16 x 8 heads x 8064 keys, 32 rows: 97 and 145, 64 rows: 190 and 147).
     const double heads_k = (double)s.batch * s.kv_heads / kKeys * 1e-3;
     const bool tiles = P.max_rows > 16 &&
                        7 + (P.max_rows + 15) / 16 * heads_k * keys_of(16) * 1.5 >

@@ -15,21 +15,23 @@
 //   warp 1          TMEM and the single-thread MMA issuer: S0_j, PV1_{j-1},
 //                   S1_j, PV0_j
 //   warps 4-7, 8-11 softmax of query tile 0 and 1, a row a thread, P kept in
-//                   TMEM, the running max raised only when a row's sum
-//                   overgrows
+//                   TMEM, the running max raised only where a tile has hidden
+//                   keys or a row's sum overgrows
 // TMEM: S0 | S1 | O0 | O1, 128 columns each; P overlays S's first 64.
 // Every wait is bounded (sm100_ptx.h).
 //
-// One frame of 1560 rows over 32760 keys x 12 heads takes 380 us (827 TFLOP/s
-// of products that are needed, half of what a large bf16 GEMM reaches), three
-// frames with a window of six and the first one kept 411, a token-causal
-// prompt of 4097 rows x 24 heads with a window of 1024 99.  A page takes a CTA
-// about 4400 cycles, 2048 of them MMAs: a query tile's S, its softmax (2300
-// cycles while the other tile's warps run theirs) and its PV follow one
-// another, and the two tiles' softmax share the SM's issue slots and MUFU.
-// Expanding the cache costs 5 %.  Measured and slower: S in halves of 64 keys
-// that land under the other half's softmax (+22 %), two threads a row (+15 %);
-// part of the exponentials on the FMA pipes gave nothing.
+// One frame of 1560 rows over 32760 keys x 12 heads takes 351 us (895 TFLOP/s
+// of products that are needed, 54 % of what a large bf16 GEMM reaches), three
+// frames with a window of six and the first one kept 369, a token-causal
+// prompt of 4097 rows x 24 heads on 8 with a window of 1024 95.  A page takes a
+// CTA about 3500 cycles, 2048 of them MMAs: a query tile's S, its exponentials
+// (1500; 1310 alone, 1024 of them MUFU's) and its PV follow one another, and
+// what lies between them counts: 240 cycles before the exponentials, 280 from
+// them to the issuer.  The roles' code shares one instruction cache: the seldom
+// paths are loops, which made the frames 3 % faster and the prompt, half of
+// whose pages have hidden keys, 2 % slower.  Measured and slower: S in halves of
+// 64 keys that land under the other half's softmax (+22 %), two threads a row
+// (+15 %), an eighth of the exponentials on the FMA pipes (+1 to 3 %).
 #include <cstring>
 
 #include "attn_kv4.cuh"
@@ -53,6 +55,7 @@ constexpr uint32_t kTileBytes = 2 * kPanel;
 constexpr int kRegsLow = 104, kRegsHigh = 200;   // warps 0-3, 4-11
 static_assert(kRegsLow * 128 + 2 * kRegsHigh * 128 <= 65536, "register split exceeds the SM");
 constexpr float kRedoSum = 32768.f;           // a tile row sum above this (2^8 shifted by kPShift) takes the new max
+constexpr float kRaise = 1.f;                  // and a score above the max by this
 constexpr int kUnits = 8;                     // of a tile: K rows 0-31, 32-63, .., then V's
 constexpr int kExpanders = 3;
 
@@ -94,9 +97,25 @@ struct __align__(1024) Smem {
 // Bits [0, n) set.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
+__device__ __forceinline__ uint32_t next_word(uint32_t (&vis)[4]) {   // four calls go round
+    const uint32_t v = vis[0];
+    vis[0] = vis[1];
+    vis[1] = vis[2];
+    vis[2] = vis[3];
+    vis[3] = v;
+    return v;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 // 128 columns of an S row of which vis says which are visible (32 a word; a
-// warp's rows agree on most words): their max, and P with its sum.  A hidden
-// key's weight is 0: everything on MUFU, whose 2^-inf is 0.
+// warp's rows agree on most words): their max, and P with its sum, word by word.
+// A hidden key's weight is 0: everything on MUFU, whose 2^-inf is 0.
 __device__ __forceinline__ void load_visible(uint32_t s_addr, uint32_t vis, uint32_t (&y)[32]) {
     KVP_TMEM_LD32(s_addr, y);
     KVP_TMEM_WAIT_LD_DEP(y);
@@ -106,11 +125,11 @@ __device__ __forceinline__ void load_visible(uint32_t s_addr, uint32_t vis, uint
             if (!(vis >> c & 1u)) y[c] = 0xFF800000u;   // -inf
     }
 }
-__device__ __forceinline__ float max_visible(uint32_t s_addr, const uint32_t (&vis)[4]) {
+__device__ __forceinline__ float max_visible(uint32_t s_addr, uint32_t (&vis)[4]) {
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
     for (int h = 0; h < 4; ++h) {
-        const uint32_t v = h == 0 ? vis[0] : h == 1 ? vis[1] : h == 2 ? vis[2] : vis[3];
+        const uint32_t v = next_word(vis);
         if (__all_sync(0xffffffffu, v == 0u)) continue;
         uint32_t y[32];
         load_visible(s_addr + 32 * h, v, y);
@@ -119,28 +138,32 @@ __device__ __forceinline__ float max_visible(uint32_t s_addr, const uint32_t (&v
     }
     return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
-__device__ __forceinline__ float exp_visible(uint32_t s_addr, float m, float sl2, const uint32_t (&vis)[4],
-                                             uint32_t (&pk)[64]) {
+// P goes to its place as it is made (columns [16 h, 16 h + 16): S's words h / 2
+// and before, which have been read).
+__device__ __forceinline__ float exp_visible(uint32_t s_addr, float m, float sl2, uint32_t (&vis)[4]) {
     float sum = 0.f;
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < 4; ++h) {
-        if (__all_sync(0xffffffffu, vis[h] == 0u)) {
+        const uint32_t v = next_word(vis);
+        uint32_t p[16];
+        if (__all_sync(0xffffffffu, v == 0u)) {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) pk[16 * h + c] = 0u;
-            continue;
-        }
-        uint32_t y[32];
-        load_visible(s_addr + 32 * h, vis[h], y);
-        float part[2] = {0.f, 0.f};
+            for (int c = 0; c < 16; ++c) p[c] = 0u;
+        } else {
+            uint32_t y[32];
+            load_visible(s_addr + 32 * h, v, y);
+            float part[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(y[c]), sl2, -m));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(y[c + 1]), sl2, -m));
-            part[0] += p0;
-            part[1] += p1;
-            pk[16 * h + (c >> 1)] = pack_f16(p0, p1);
+            for (int c = 0; c < 32; c += 2) {
+                const float p0 = ex2_approx(fmaf(__uint_as_float(y[c]), sl2, -m));
+                const float p1 = ex2_approx(fmaf(__uint_as_float(y[c + 1]), sl2, -m));
+                part[0] += p0;
+                part[1] += p1;
+                p[c >> 1] = pack_f16(p0, p1);
+            }
+            sum += part[0] + part[1];
         }
-        sum += part[0] + part[1];
+        tmem_st16(s_addr + 16 * h, p);
     }
     return sum;
 }
@@ -559,8 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 for (int k = 0; k < 32; k += 2) {
                     const bool in = rw + sub + k < rows;
                     const RowOf y = row_of(P, qi0, qg0, mine0 + sub + k);
-                    cp_async16(dst + sw128_off((warp & 3) * 32 + sub + k, chunk & 7),
-                               in ? src + y.row * P.attn.q_row_stride + (long long)y.g * kKv4Head : P.attn.q, in ? 16u : 0u);
+                    const __nv_bfloat16* at = src + y.row * P.attn.q_row_stride + (long long)y.g * kKv4Head;
+                    cp_async16(dst + sw128_off((warp & 3) * 32 + sub + k, chunk & 7), in ? at : P.attn.q,
+                               in ? 16u : 0u);
                 }
                 cp_async_wait_all();
                 fence_proxy_async_smem();
@@ -613,10 +637,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                 // the low half.  Nearly every tile goes the first way, against the
                 // running max, which is laid out without a jump (700 cycles stood
                 // between S and the first exponential before).
-                uint32_t pk[64];
                 float rsum = 0.f;
-                bool done = plain;
                 if (__builtin_expect(plain, 1)) {
+                    uint32_t pk[64];
                     rsum = exp_row<false, 4, 0u, true>(s_tm, m_run - kPShift, P.scale_log2, kBN, pk);
                     if (__builtin_expect(some_gone, 0)) {
                         if (gone) {
@@ -625,24 +648,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                             for (int c = 0; c < 64; ++c) pk[c] = 0u;
                         }
                     }
-                    done = __all_sync(0xffffffffu, rsum <= kRedoSum);
-                }
-                if (__builtin_expect(!done, 0)) {
-                    // Hidden keys, a row's first key (the max comes first then) or a
-                    // row whose sum overgrows (it takes the tile's max and goes again).
-                    const bool first = __any_sync(0xffffffffu, m_run == -INFINITY && !gone);
-                    float m_new = m_run;
-#pragma unroll 1
-                    for (int pass = first || plain ? 1 : 0; pass < 2; ++pass) {
-                        if (pass == 1) {
-                            const bool raise = !gone && (first || !(rsum <= kRedoSum));
-                            if (!__any_sync(0xffffffffu, raise)) break;
-                            const float top = max_visible(s_tm, vis);
-                            if (raise) m_new = fmaxf(m_run, top * P.scale_log2);
-                        }
-                        // (a row without keys keeps max -inf: subtract 0)
-                        rsum = exp_visible(s_tm, (m_new == -INFINITY ? 0.f : m_new) - kPShift, P.scale_log2, vis, pk);
+                    plain = __all_sync(0xffffffffu, rsum <= kRedoSum);
+                    if (__builtin_expect(plain, 1)) {
+                        KVP_TMEM_ST32(s_tm, pk);
+                        KVP_TMEM_ST32(s_tm + 32, (pk + 32));
                     }
+                }
+                if (__builtin_expect(!plain, 0)) {
+                    // Hidden keys, a row's first key or a sum that overgrows (some
+                    // score is above the max by 1 then): the tile's max first.
+                    const float top = max_visible(s_tm, vis) * P.scale_log2;
+                    const float m_new = top > m_run + kRaise ? top : m_run;
+                    // (a row without keys keeps max -inf: subtract 0)
+                    rsum = exp_visible(s_tm, (m_new == -INFINITY ? 0.f : m_new) - kPShift, P.scale_log2, vis);
                     const float alpha = m_new == m_run ? 1.f : ex2_approx(m_run - m_new);
                     l_run *= alpha;
                     m_run = m_new;
@@ -662,8 +680,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                     }
                 }
                 l_run += rsum;
-                KVP_TMEM_ST32(s_tm, pk);
-                KVP_TMEM_ST32(s_tm + 32, (pk + 32));
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&sm.bar_p_full[qt]);
