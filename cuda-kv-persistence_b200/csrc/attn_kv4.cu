@@ -610,15 +610,37 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
     long long grid = units, slots = 0;   // slots: rows of the workspace
     const long long keys = keys_of(tile_rows);
     if (tiles) {
-        // A CTA an SM takes one unit after the other.  Units that do not divide
-        // evenly over the SMs are cut: the CTAs share all units' pages, which
-        // costs a piece more for each (about three pages) and the join (three).
+        // Units whose number does not divide over the SMs can be cut: the CTAs
+        // share all units' pages evenly, for two pieces more a CTA, their partial
+        // rows and the join, about 6 pages' time and a twentieth for each unit (12
+        // heads x 1560 rows over 9360 keys, 84 units: 121 us, whole 167; over 3120
+        // keys 60 and 63; 8 x 3 heads x 2000 rows, causal, 192 units: 72 and 45; 3
+        // frames over 10920 of 12 heads, 228 units: 367 and 430).  Whole units,
+        // longest first, take as long as the longest of each round, or the even
+        // share and what the last ones stick out.
         P.splits = 1;
-        const long long sms = sm_count(), pages = (keys + kKv4PageRows - 1) / kKv4PageRows;
-        P.chunked = (units + sms - 1) / sms * (pages + 3) > units * (pages + 3) / sms + 6 && units < 8 * sms &&
-                    (long long)s.batch * P.row_tiles <= kKv4ChunkPairs && units * s.map_stride < 0x7fffffffLL;
+        const int sms = sm_count();
+        const long long start = s.starts ? std::max(0LL, cap - s.rows) : s.start, pairs = (long long)s.batch * P.row_tiles;
+        auto cost = [&](long long unit) {             // of a unit in the list (unit_of)
+            const long long r0 = (P.row_tiles - 1 - unit / s.kv_heads / s.batch) * 256;
+            const long long f0 = (start + r0 / P.group) / a.tokens * a.tokens + a.tokens;
+            const long long last = start + (std::min<long long>(r0 + 256, P.max_rows) - 1) / P.group;
+            const long long f1 = last / a.tokens * a.tokens + a.tokens;
+            const long long lo = P.window_rows ? std::max(0LL, f0 - P.window_rows) / kKv4PageRows : 0;
+            const long long hi = (std::min(f1, start + s.rows) + kKv4PageRows - 1) / kKv4PageRows;
+            return hi - lo + std::min<long long>((P.sink_rows + kKv4PageRows - 1) / kKv4PageRows, lo) + kKv4UnitCost;
+        };
+        constexpr int kSamples = 16;
+        double share = 0, rounds = 0;
+        for (int i = 0; i < kSamples; ++i) share += (double)cost((2 * i + 1) * units / (2 * kSamples));
+        share *= (double)units / (kSamples * sms);
+        if (units < 8 * sms)
+            for (long long u = 0; u < units; u += sms) rounds += (double)cost(u);
+        P.chunked = units < 8 * sms && pairs <= kKv4ChunkPairs &&
+                    units * (s.map_stride + kKv4UnitCost) < 0x7fffffffLL &&
+                    std::min(rounds, share + (double)cost(units - 1)) > share + 6 + units / 20.0;
         if (P.chunked) {
-            grid = sm_count();
+            grid = sms;
             slots = 2 * 256 * grid;
             // eight CTAs an SM, at least sixteen a unit (few units are in many pieces)
             P.join_ctas = (int)std::max(16LL, std::min(128LL, 8 * sms / units));

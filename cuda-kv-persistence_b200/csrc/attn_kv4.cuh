@@ -14,7 +14,7 @@ struct Kv4Params {
     int* status;
     float* ws_o;             // partial O of split c: [sequence][K/V head][row][split][128]
     float* ws_ml;            // its max (log2 units) and sum: [...][split][2]
-    int* ws_unit;            // chunked: [0] pages of a CTA, [1 + unit] the unit's first page in the list of all
+    int* ws_unit;            // chunked: [0] a CTA's share, [1 + unit] where the unit's first page is in the list
     long long window_rows;   // window * tokens (0: all keys)
     int sink_rows;           // sinks * tokens, at most the capacity
     int group, max_rows;     // query heads per K/V head; rows * group
@@ -51,13 +51,16 @@ __device__ __forceinline__ __nv_bfloat16* out_row(const Kv4Params& P, int b, int
            (long long)(r / P.group) * P.attn.out_row_stride + (long long)(h * P.group + r % P.group) * kKv4Head;
 }
 
+constexpr int kKv4UnitCost = 3;
+
 // The units of the kernel for many rows: 256 query rows of one sequence and
 // K/V head, against the pages that any of them sees (those of the sinks
 // below the window, then the window's).  Unit u = pair * kv_heads + head,
 // pairs of (row tile, sequence) with the last rows, the longest spans, first.
-// Chunked, CTA i takes pages [i C, (i + 1) C) of the list of all units' pages;
-// a piece that is not its whole unit is a partial, in slot 2 i + 1 if it
-// begins the unit (it is the CTA's last then), 2 i if not (its first).
+// Chunked, CTA i takes [i C, (i + 1) C) of the list of all units' costs, a unit's
+// being kKv4UnitCost (what its beginning and end take, in pages' time) and then
+// its pages; a piece that is not its whole unit is a partial, in slot 2 i + 1 if
+// it begins the unit (it is the CTA's last then), 2 i if not (its first).
 struct Kv4Unit {
     int b, start, end, rows, r0;       // rows = count * group; this unit's [r0, r0 + 256)
     int na, b0, pages;                 // pages [0, na) and [b0, b0 + pages - na); 0: nothing to do

@@ -59,8 +59,9 @@ constexpr float kRaise = 1.f;                  // and a score above the max by t
 constexpr int kUnits = 8;                     // of a tile: K rows 0-31, 32-63, .., then V's
 constexpr int kExpanders = 3;
 
-// Where a CTA is in its list of units, and the pages it still takes.  Each role
-// holds its own and moves it on by itself.
+// Where a CTA is in its list of units, in costs: a unit costs kKv4UnitCost and
+// its pages.  off: in the unit, left: what the CTA still takes, pos: in the list.
+// Each role holds its own and moves it on by itself.
 struct Work {
     int pair, head, off, left, pos;
 };
@@ -185,7 +186,7 @@ __device__ __forceinline__ void expand4(uint8_t* tile, const uint32_t (&off)[4],
     *reinterpret_cast<uint4*>(tile + off[3]) = values(w3, s23);
 }
 
-constexpr int kMinPages = 2;                  // of a CTA's share: a piece costs about three pages more
+constexpr int kMinPages = 2;                  // of a CTA's share, beside a unit's own cost
 
 __device__ __forceinline__ void init_barriers(Smem& sm) {
     for (int q = 0; q < 2; ++q) {
@@ -220,8 +221,8 @@ struct Piece {
     bool two;                                 // the second query tile has rows
     __device__ __forceinline__ Piece(const Kv4Params& P, const Work& w) {
         u = unit_of(P, w.pair);
-        u0 = w.off;
-        n_tiles = min(u.pages - u0, w.left);
+        u0 = max(w.off - kKv4UnitCost, 0);
+        n_tiles = max(min(w.off + w.left - kKv4UnitCost, u.pages) - u0, 0);   // (0: the list ends before the first page)
         two = u.r0 + 128 < u.rows;
         rot = free0() < free1() ? free0() : 0;
     }
@@ -237,10 +238,11 @@ struct Piece {
     }
 };
 
-// The next piece of the list after one of n_tiles.
-__device__ __forceinline__ void advance(const Kv4Params& P, Work& w, int n_tiles) {
-    w.left -= n_tiles;
-    w.pos += n_tiles;
+// The next piece of the list after one of a unit of `pages`.
+__device__ __forceinline__ void advance(const Kv4Params& P, Work& w, int pages) {
+    const int cost = min(kKv4UnitCost + pages - w.off, w.left);
+    w.left -= cost;
+    w.pos += cost;
     w.off = 0;
     if (++w.head == P.span.kv_heads && w.left > 0) {
         w.head = 0;
@@ -274,13 +276,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
     // Where this CTA's work begins, and how many pages it takes.
     int left = 0;
     if (P.chunked) {
-        // prefix sums of the pairs' pages, three pairs a thread
+        // prefix sums of the pairs' costs, three pairs a thread
         const int pairs = P.row_tiles * s.batch;
         int n[3], mine = 0;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
             const int p = 3 * (int)threadIdx.x + i;
             n[i] = p < pairs ? unit_of(P, p).pages : 0;
+            if (n[i] > 0) n[i] += kKv4UnitCost;
             mine += n[i];
         }
         int upto = mine;
@@ -297,13 +300,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             all += sm.scan[w];
         }
         all *= s.kv_heads;
-        const int chunk = max((all + (int)gridDim.x - 1) / (int)gridDim.x, kMinPages);
+        const int chunk = max((all + (int)gridDim.x - 1) / (int)gridDim.x, kKv4UnitCost + kMinPages);
         const int pos = (int)min((long long)blockIdx.x * chunk, (long long)all);
         left = min(chunk, all - pos);
         if (blockIdx.x == 0 && threadIdx.x == 0) P.ws_unit[0] = chunk;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-            const int r = pos - before * s.kv_heads;   // pages into this pair's kv_heads units
+            const int r = pos - before * s.kv_heads;   // into this pair's kv_heads units
             if (left > 0 && r >= 0 && r < n[i] * s.kv_heads) {
                 sm.first = Work{3 * (int)threadIdx.x + i, r / n[i], r % n[i], left, pos};
             }
@@ -312,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
     } else {
         const int pair = (int)(blockIdx.x / (uint32_t)s.kv_heads);
         left = unit_of(P, pair).pages;
+        if (left > 0) left += kKv4UnitCost;
         if (threadIdx.x == 0) sm.first = Work{pair, (int)(blockIdx.x % (uint32_t)s.kv_heads), 0, left, 0};
     }
     // the refused sequences are reported once
@@ -361,6 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
             int turn = 0;
             for (int tile0 = 0; ok && w.left > 0;) {
                 const Piece pc(P, w);
+                if (pc.n_tiles == 0) break;
                 if (warp == 0) ok = next_turn(turn);
                 if (!ok) break;
                 if (warp == 0 && lane == 0) {
@@ -382,7 +387,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                     t.tile0 = tile0;
                     t.qi0 = pc.u.r0 / P.group;
                     t.qg0 = pc.u.r0 % P.group;
-                    if (P.chunked && w.off == 0) P.ws_unit[1 + w.pair * s.kv_heads + w.head] = w.pos;
+                    if (P.chunked && pc.u0 == 0)
+                        P.ws_unit[1 + w.pair * s.kv_heads + w.head] = w.pos - w.off + kKv4UnitCost;
                     mbar_arrive(&sm.bar_turn[turn % kTurns]);
                 }
                 ++turn;
@@ -455,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                     if (lane == 0) mbar_arrive(part ? &sm.bar_vfull[st] : &sm.bar_kfull[st]);
                 }
                 tile0 += pc.n_tiles;
-                advance(P, w, pc.n_tiles);
+                advance(P, w, pc.u.pages);
             }
             if (warp == 0 && ok && next_turn(turn) && lane == 0) {
                 sm.turn[turn % kTurns].n_tiles = 0;
@@ -479,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                     const Piece pc(P, w);
                     const int n_tiles = pc.n_tiles;
                     const bool two = pc.two;
+                    if (n_tiles == 0) break;
                     ok = mbar_wait(&sm.bar_q[0], q0_ph, sm, P.status);
                     if (ok && two) ok = mbar_wait(&sm.bar_q[1], q1_ph, sm, P.status);
                     bool k_known = false;
@@ -536,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __gri
                         }
                         q0_ph ^= 1u;
                     }
-                    advance(P, w, n_tiles);
+                    advance(P, w, pc.u.pages);
                 }
                 // Drain: every issued MMA lands before TMEM is freed.
                 tc_commit(&sm.bar_mma_done);

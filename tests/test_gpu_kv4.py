@@ -451,6 +451,22 @@ def test_strided_queries_and_the_same_call_twice(rows, heads):
     assert bool((a[..., heads * 128:] == 7).all())
 
 
+@pytest.mark.parametrize("kw", [{}, dict(window=700, sinks=150), dict(tokens=90, window=4, sinks=1)])
+def test_many_units_cut_where_they_do_not_divide(kw):
+    """150 units of 12 pages: each CTA goes from one sequence's or head's to
+    the next; one and two query tiles, sequences of no rows between them."""
+    rng = np.random.default_rng(len(kw))
+    batch, kvh, rows, per = 15, 10, 130, 12
+    starts = [per * 128 - rows - int(x) for x in rng.integers(0, 400, batch)]
+    counts = [int(x) for x in rng.choice([rows, rows, 100, 129, 7, 0], batch)]
+    starts[3], counts[3] = 0, rows
+    pages = _calm_pool(rng, batch * per, kvh)
+    got, want, tol = _attend(rng, pages, _map(rng, batch, per, batch * per), starts, counts, rows, kvh,
+                             use=("starts", "counts"), **kw)
+    _check(got, want, tol)
+    assert _status() == 0
+
+
 @pytest.mark.parametrize("rows", [1, 3, 130])
 def test_sequences_inside_rows_in_place_and_shared_queries(rows):
     """Row-major batches ([rows, batch, ...] seen as [batch, rows, ...]) in
