@@ -24,7 +24,8 @@ import struct
 
 import torch
 
-from ._lib import KvpError, check, lib
+from . import KvpError
+from ._lib import check, lib
 
 PAGE_ROWS = 128
 PAGE_HEAD_BYTES = 18432
