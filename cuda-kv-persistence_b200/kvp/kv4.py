@@ -38,9 +38,11 @@ _MAX_INT = 2 ** 31
 _SPAN = struct.Struct("@PPPPqiiiii4x").pack
 _ROWS = struct.Struct("@PPqqi4x").pack
 _ATTN = struct.Struct("@PPqqqqiiii").pack
-# the current stream's handle without building a Stream object
+# the current stream's handle without building a Stream object, the current
+# device without asking whether CUDA is up (a tensor is on it)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def alloc_pages(n_pages: int, kv_heads: int, device="cuda"):
@@ -52,50 +54,58 @@ def _bad(what: str):
     raise KvpError(f"kv4: {what}")
 
 
-def _rows3(t, name: str, dtypes, heads: int):
-    """(batch, rows, row stride, batch stride) of a row tensor."""
-    if t.dtype not in dtypes:
-        _bad(f"{name} is {t.dtype}, expected one of {[str(d) for d in dtypes]}")
-    shape, strides = t.shape, t.stride()
-    if len(shape) == 3:
-        b, n, d = shape
-        bs, rs, es = strides
-    elif len(shape) == 2:
-        n, d = shape
-        rs, es = strides
-        b, bs = 1, 0
-    else:
-        _bad(f"{name} must be [rows, heads * 128] or [batch, rows, heads * 128]")
-    if d != heads * 128 or es != 1:
-        _bad(f"{name} needs {heads} heads of 128 contiguous elements, got {tuple(shape)}")
-    # the strides of single rows and sequences mean nothing
-    return b, n, rs if n > 1 else d, bs if b > 1 else 0
-
-
-def _pool(pages):
-    """(n_pages, kv_heads) of a pool."""
-    shape = pages.shape
-    if len(shape) != 3 or shape[2] != PAGE_HEAD_BYTES or pages.dtype != torch.uint8 or \
-            not pages.is_contiguous():
-        _bad(f"pages must be a contiguous uint8 [n_pages, kv_heads, {PAGE_HEAD_BYTES}] tensor")
-    return shape[0], shape[1]
-
-
 def _ints(t, name: str, batch: int, dev: int, dims: int) -> int:
-    if t.dtype != torch.int32 or t.dim() != dims or t.shape[0] != batch or not t.is_contiguous():
+    shape = t.shape
+    if t.dtype is not torch.int32 or len(shape) != dims or shape[0] != batch or not t.is_contiguous():
         _bad(f"{name} must be a contiguous int32 [{batch}{', pages' if dims == 2 else ''}] tensor")
     if t.get_device() != dev:
         _bad(f"tensors on {t.device} and cuda:{dev}")
     return t.data_ptr()
 
 
-def _span(pages, n_pages, kv_heads, batch: int, rows: int, page_map, start: int, starts, counts, a, b):
+def _args(pages, a, b, names: str, types, heads, page_map, start: int, starts, counts):
+    """Checks the pool, the row tensors a and b (b may be None; heads None: the
+    pool's) and the rest; (device, packed span, a's row and batch stride, b's).
+    One function, because calls of several cost a microsecond of the seven that
+    a call of the package takes."""
+    shape = pages.shape
+    if len(shape) != 3 or shape[2] != PAGE_HEAD_BYTES or pages.dtype is not torch.uint8 or \
+            not pages.is_contiguous():
+        _bad(f"pages must be a contiguous uint8 [n_pages, kv_heads, {PAGE_HEAD_BYTES}] tensor")
+    n_pages, kv_heads, _ = shape
+    width = (kv_heads if heads is None else heads) * 128
+    shape, strides, dtype = a.shape, a.stride(), a.dtype
+    if dtype not in types:
+        _bad(f"{names} of {dtype}, expected one of {[str(d) for d in types]}")
+    if len(shape) == 3:
+        batch, rows, d = shape
+        bs, rs, es = strides
+    elif len(shape) == 2:
+        batch, bs = 1, 0
+        rows, d = shape
+        rs, es = strides
+    else:
+        _bad(f"{names} must be [rows, heads * 128] or [batch, rows, heads * 128]")
+    if d != width or es != 1:
+        _bad(f"{names} need {width // 128} heads of 128 contiguous elements, got {tuple(shape)}")
+    b_rs, b_bs = rs, bs
+    if b is not None:
+        if b.dtype is not dtype or b.shape != shape:
+            _bad(f"{names} must agree in shape and type")
+        if (other := b.stride()) != strides:
+            if other[-1] != 1:
+                _bad(f"{names} need {width // 128} heads of 128 contiguous elements")
+            b_rs, b_bs = other[-2], other[0] if len(other) == 3 else 0
+    # the strides of single rows and sequences mean nothing
+    if rows < 2:
+        rs = b_rs = width
+    if batch < 2:
+        bs = b_bs = 0
     dev = pages.get_device()
     if dev < 0:
         _bad("pages must be a CUDA tensor")
-    for t in (a, b):
-        if t is not None and t.get_device() != dev:
-            _bad(f"tensors on {t.device} and cuda:{dev}")
+    if a.get_device() != dev or (b is not None and b.get_device() != dev):
+        _bad(f"tensors on {a.device if b is None else f'{a.device}, {b.device}'} and cuda:{dev}")
     if page_map is None:
         stride, map_ptr = n_pages // max(batch, 1), 0
     else:
@@ -106,11 +116,11 @@ def _span(pages, n_pages, kv_heads, batch: int, rows: int, page_map, start: int,
     return dev, _SPAN(pages.data_ptr(), map_ptr,
                       0 if starts is None else _ints(starts, "starts", batch, dev, 1),
                       0 if counts is None else _ints(counts, "counts", batch, dev, 1),
-                      n_pages, kv_heads, batch, stride, start, rows)
+                      n_pages, kv_heads, batch, stride, start, rows), rs, bs, b_rs, b_bs
 
 
 def _call(fn, what, dev, stream, span, args):
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = fn(span, args, _raw_stream(dev) if stream is None else stream)
     else:
         with torch.cuda.device(dev):
@@ -120,15 +130,13 @@ def _call(fn, what, dev, stream, span, args):
 
 
 def _kv(pages, k, v, page_map, start, starts, counts):
-    some = k if k is not None else v
+    some, other = (k, v) if k is not None else (v, None)
     if some is None:
         _bad("no rows")
-    n_pages, heads = _pool(pages)
-    b, n, rs, bs = shape = _rows3(some, "k" if k is not None else "v", _ROW_TYPES, heads)
-    if k is not None and v is not None and (_rows3(v, "v", _ROW_TYPES, heads) != shape or
-                                            k.dtype != v.dtype):
-        _bad("k and v must agree in shape, strides and type")
-    dev, span = _span(pages, n_pages, heads, b, n, page_map, start, starts, counts, k, v)
+    dev, span, rs, bs, v_rs, v_bs = _args(pages, some, other, "k and v", _ROW_TYPES, None, page_map, start, starts,
+                                          counts)
+    if rs != v_rs or bs != v_bs:
+        _bad("k and v must agree in strides")
     return dev, span, _ROWS(0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), rs, bs,
                             some.element_size())
 
@@ -156,12 +164,8 @@ def attn(q, pages, out, *, heads: int, page_map=None, start: int = 0, starts=Non
     its frame (and of this call's rows) that lie in the last `window` frames
     (0: all) or the first `sinks` frames.  The call's own rows are keys: write
     them first.  out may be q."""
-    n_pages, kv_heads = _pool(pages)
-    b, n, qr, qb = _rows3(q, "q", _Q_TYPES, heads)
-    ob, on, orow, obatch = _rows3(out, "out", _Q_TYPES, heads)
-    if ob != b or on != n:
-        _bad("q and out must agree in shape")
-    dev, span = _span(pages, n_pages, kv_heads, b, n, page_map, start, starts, counts, q, out)
+    dev, span, qr, qb, orow, obatch = _args(pages, q, out, "q and out", _Q_TYPES, heads, page_map, start, starts,
+                                            counts)
     if not (0 < tokens < _MAX_INT and 0 <= window < _MAX_INT and 0 <= sinks < _MAX_INT):
         _bad(f"tokens {tokens}, window {window} or sinks {sinks} out of range")
     _call(lib().kvp_attn_kv4, "kvp_attn_kv4", dev, stream, span,
