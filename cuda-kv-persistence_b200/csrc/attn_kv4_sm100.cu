@@ -265,7 +265,8 @@ __device__ __forceinline__ RowOf row_of(const Kv4Params& P, int qi0, int qg0, in
 
 __global__ void __launch_bounds__(kThreads, 1) attn_kv4_sm100_kernel(const __grid_constant__ Kv4Params P) {
     extern __shared__ uint8_t smem_raw[];
-    cudaTriggerProgrammaticLaunchCompletion();    // the join may be launched; it waits for the data
+    cudaGridDependencySynchronize();              // (kv4_config)
+    if (P.chunked) cudaTriggerProgrammaticLaunchCompletion();   // the join may be launched; it waits for the data
     if (reinterpret_cast<uintptr_t>(smem_raw) & 1023) {
         if (threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_ALIGN);
         return;
@@ -796,8 +797,9 @@ int launch_kv4_tiles(const Kv4Params& P, unsigned grid, cudaStream_t stream) {
         return KVP_OK;
     });
     if (rc != KVP_OK) return rc;
-    attn_kv4_sm100_kernel<<<grid, kThreads, smem, stream>>>(P);
-    KVP_CUDA(cudaGetLastError());
+    cudaLaunchAttribute early;
+    const cudaLaunchConfig_t cfg = kv4_config(grid, kThreads, (size_t)smem, &early, stream);
+    KVP_CUDA(cudaLaunchKernelEx(&cfg, attn_kv4_sm100_kernel, P));
     return KVP_OK;
 }
 

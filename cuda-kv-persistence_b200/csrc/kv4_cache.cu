@@ -136,11 +136,12 @@ __device__ __forceinline__ uint32_t quantise16(uint32_t (&x)[8], uint32_t (&word
 
 template <class T>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
-    kv4_write_kernel(const Kv4Span s, const T* __restrict__ k, const T* __restrict__ v, long long row_stride,
-                     long long batch_stride, int blocks, long long items, int* status) {
+    kv4_write_kernel(const Kv4Span s, T* k, T* v, long long row_stride, long long batch_stride, int blocks,
+                     long long items, int* status) {
     __shared__ __align__(16) uint8_t stage[sizeof(T) == 4 ? kThreads / 32 : 1][4096];
     const int lane = threadIdx.x & 31;
     const long long step = (long long)gridDim.x * (kThreads / 32);
+    cudaGridDependencySynchronize();                  // (kv4_config)
     for (long long w = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < items; w += step) {
         Item it;
         if (!item_of(s, w, blocks, lane, status, it) || !it.blk) continue;
@@ -223,14 +224,14 @@ struct Out<float> {
 };
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const Kv4Span s, T* __restrict__ k,
-                                                            T* __restrict__ v, long long row_stride,
-                                                            long long batch_stride, int blocks,
-                                                            long long items, int* status) {
+__global__ void __launch_bounds__(kThreads)
+    kv4_read_kernel(const Kv4Span s, T* k, T* v, long long row_stride, long long batch_stride, int blocks,
+                    long long items, int* status) {
     constexpr int kDims = Out<T>::kDims, kLanes = 128 / kDims, kRows = 32 / kLanes;   // lanes of a row, rows of a pass
     const int lane = threadIdx.x & 31;
     const int dim = lane % kLanes * kDims, word = dim / 8, part = dim % 8 / 4;
     const long long step = (long long)gridDim.x * (kThreads / 32);
+    cudaGridDependencySynchronize();                  // (kv4_config)
     for (long long w = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < items; w += step) {
         Item it;
         if (!item_of(s, w, blocks, lane, status, it)) continue;
@@ -305,16 +306,20 @@ bool apart(const Kv4Span& s, long long row_stride, long long batch_stride, long 
            row_stride >= (s.batch - 1) * batch_stride + len;
 }
 
-template <class K>
-int launch(const Kv4Span& s, cudaStream_t stream, K&& kernel) {
+template <class Row>
+int launch(const Kv4Span& s, const Kv4Rows& r, int* status, cudaStream_t stream,
+           void (*kernel)(Kv4Span, Row*, Row*, long long, long long, int, long long, int*)) {
     // rows may begin anywhere in a block: the last row's block is
     // (start % 8 + rows - 1) / 8 blocks after the first
     const int lead = s.starts ? kKv4BlockRows - 1 : s.start % kKv4BlockRows;
     const int blocks = (int)(((long long)lead + s.rows + kKv4BlockRows - 1) / kKv4BlockRows);
     const long long items = (long long)s.batch * s.kv_heads * blocks;
     const long long ctas = (items + kThreads / 32 - 1) / (kThreads / 32);
-    kernel(blocks, items, (unsigned)(ctas < 0x7fffffffLL ? ctas : 0x7fffffffLL));
-    KVP_CUDA(cudaGetLastError());
+    cudaLaunchAttribute early;
+    const cudaLaunchConfig_t cfg =
+        kv4_config((unsigned)(ctas < 0x7fffffffLL ? ctas : 0x7fffffffLL), kThreads, 0, &early, stream);
+    KVP_CUDA(cudaLaunchKernelEx(&cfg, kernel, s, static_cast<Row*>(r.k), static_cast<Row*>(r.v), r.row_stride,
+                                r.batch_stride, blocks, items, status));
     return KVP_OK;
 }
 
@@ -374,29 +379,15 @@ int check_kv4_attn(const Kv4Span& s, const Kv4Attn& a) {
 int launch_kv4_write(const Kv4Span& s, const Kv4Rows& r, int* d_status, cudaStream_t stream) {
     const int rc = check_kv4_rows(s, r, true);
     if (rc != KVP_OK || s.rows == 0 || s.batch == 0) return rc;
-    return launch(s, stream, [&](int blocks, long long items, unsigned ctas) {
-        if (r.elem_bytes == 2)
-            kv4_write_kernel<__nv_bfloat16><<<ctas, kThreads, 0, stream>>>(
-                s, (const __nv_bfloat16*)r.k, (const __nv_bfloat16*)r.v, r.row_stride, r.batch_stride, blocks,
-                items, d_status);
-        else
-            kv4_write_kernel<float><<<ctas, kThreads, 0, stream>>>(
-                s, (const float*)r.k, (const float*)r.v, r.row_stride, r.batch_stride, blocks, items, d_status);
-    });
+    return r.elem_bytes == 2 ? launch(s, r, d_status, stream, kv4_write_kernel<__nv_bfloat16>)
+                             : launch(s, r, d_status, stream, kv4_write_kernel<float>);
 }
 
 int launch_kv4_read(const Kv4Span& s, const Kv4Rows& r, int* d_status, cudaStream_t stream) {
     const int rc = check_kv4_rows(s, r, false);
     if (rc != KVP_OK || s.rows == 0 || s.batch == 0) return rc;
-    return launch(s, stream, [&](int blocks, long long items, unsigned ctas) {
-        if (r.elem_bytes == 2)
-            kv4_read_kernel<__nv_bfloat16><<<ctas, kThreads, 0, stream>>>(
-                s, (__nv_bfloat16*)r.k, (__nv_bfloat16*)r.v, r.row_stride, r.batch_stride, blocks, items,
-                d_status);
-        else
-            kv4_read_kernel<float><<<ctas, kThreads, 0, stream>>>(
-                s, (float*)r.k, (float*)r.v, r.row_stride, r.batch_stride, blocks, items, d_status);
-    });
+    return r.elem_bytes == 2 ? launch(s, r, d_status, stream, kv4_read_kernel<__nv_bfloat16>)
+                             : launch(s, r, d_status, stream, kv4_read_kernel<float>);
 }
 
 }  // namespace kvp

@@ -371,7 +371,8 @@ int kvp_kv4_read(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream);
  * min((f + 1) * tokens, start + count) that are in frames f - window + 1 ..
  * f or in the first `sinks` frames.  (The call's own rows are keys too: write
  * them first.)  A row that sees no key is 0; one of q that is not finite
- * spoils its own output only.  out may be q, with the same strides.  One row
+ * spoils its own output only, and so may one with scores |q . k| beyond 2^26,
+ * where fp32's spacing passes what the softmax can hold.  out may be q, with the same strides.  One row
  * per sequence is a decoding step, tokens = 1 a causal prompt, tokens = 1560 a
  * video frame.  Keys that are split over several CTAs are joined through a
  * workspace from the private, stream-ordered memory pool. */

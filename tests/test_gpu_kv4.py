@@ -550,6 +550,38 @@ def test_graphs_replay_and_do_not_share_workspaces(rows, far):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("rows,start", [(1, 300), (1, 4000), (1, 9000), (40, 900), (300, 700), (300, 9000)])
+@pytest.mark.parametrize("wait", [False, True])
+def test_calls_follow_one_another(rows, start, wait):
+    """Kernels are launched before what precedes them ends: rows, queries, starts,
+    pages and outputs that the call before, or another kernel, has just written
+    or read.  With and without a wait in between the results are the same."""
+    from kvp import kv4
+    gen = torch.Generator(device="cuda").manual_seed(rows + start)
+    pages = kv4.alloc_pages(80, 2).random_(0, 256, generator=gen)
+    x = torch.randn(20, rows, 256, device="cuda", generator=gen).to(BF)
+    results = []
+    for pause in (True, wait):
+        p, q = pages.clone(), torch.zeros(rows, 512, dtype=BF, device="cuda")
+        k, v = (torch.zeros_like(x[0]) for _ in range(2))
+        at = torch.full((1,), start, dtype=torch.int32, device="cuda")
+        out, back, outs = torch.zeros_like(q), torch.zeros_like(x[0]), []
+        torch.cuda.synchronize()
+        for i in range(20):
+            for step in (lambda: k.copy_(x[i]), lambda: v.copy_(x[19 - i]), lambda: q.copy_(x[i].repeat(1, 2)),
+                         lambda: kv4.write(p, k, v, starts=at), lambda: kv4.attn(q, p, out, heads=4, starts=at),
+                         lambda: q.copy_(out), lambda: kv4.attn(q, p, q, heads=4, starts=at),
+                         lambda: kv4.write(p, q[:, :256], q[:, 256:], starts=at),
+                         lambda: kv4.read(p, back, None, starts=at),
+                         lambda: outs.append(torch.cat((out, q, back), 1)), lambda: at.add_(i % 3 - 1)):
+                step()
+                if pause:
+                    torch.cuda.synchronize()
+        results.append(torch.stack(outs).view(torch.int16))       # (bits: arbitrary bytes make scores that overflow)
+    assert torch.equal(results[0], results[1])
+    assert _status() in (0, 8)          # some of them are written back, beyond the format
+
+
 def test_two_streams_at_once():
     from kvp import kv4
     rng = np.random.default_rng(16)
