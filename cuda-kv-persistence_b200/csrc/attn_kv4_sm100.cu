@@ -20,10 +20,10 @@
 // TMEM: S0 | S1 | O0 | O1, 128 columns each; P overlays S's first 64.
 // Every wait is bounded (sm100_ptx.h).
 //
-// One frame of 1560 rows over 32760 keys x 12 heads takes 346 us (907 TFLOP/s
-// of products that are needed, 54 % of what a large bf16 GEMM reaches), three
+// One frame of 1560 rows over 32760 keys x 12 heads takes 344 us (913 TFLOP/s
+// of products that are needed, 55 % of what a large bf16 GEMM reaches), three
 // frames with a window of six and the first one kept 366, a token-causal
-// prompt of 4097 rows x 24 heads on 8 with a window of 1024 95.  A page takes a
+// prompt of 4097 rows x 24 heads on 8 with a window of 1024 94.6.  A page takes a
 // CTA about 3500 cycles, 2048 of them MMAs: a query tile's S, its exponentials
 // (1500; 1310 alone, 1024 of them MUFU's) and its PV follow one another, and
 // what lies between them counts: 240 cycles before the exponentials, 280 from
