@@ -658,7 +658,7 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
         const long long want = std::max<long long>(1, std::min(at_once[0] / units, most));
         // Splits that are a cluster join without workspace and second launch,
         // which is worth two steps more a warp (4099 keys x 12 heads: 8 in a
-        // cluster 8.0 us at 6 us of host time, 12 and a join 8.4 at 10;
+        // cluster 8.0 us, 12 and a join 8.4 and a second launch's host time;
         // 16 sequences of 8191 x 8 heads: 2 in a cluster 34.4, 2 and a join
         // 36.3; 32768 x 12 heads: 8 in a cluster 27.2, 24 and a join 20.0).
         auto a_warp = [&](long long c) { return (steps + c * kWarps - 1) / (c * kWarps); };

@@ -28,7 +28,7 @@
 // (1500; 1310 alone, 1024 of them MUFU's) and its PV follow one another, and
 // what lies between them counts: 240 cycles before the exponentials, 280 from
 // them to the issuer.  The roles' code shares one instruction cache: the seldom
-// paths are loops, which made the frames 3 % faster and the prompt, half of
+// paths are loops, which made the frames 3 % faster and the prompt, a third of
 // whose pages have hidden keys, 2 % slower.  Measured and slower: S in halves of
 // 64 keys that land under the other half's softmax (+22 %), two threads a row
 // (+15 %), an eighth of the exponentials on the FMA pipes (+1 to 3 %).
