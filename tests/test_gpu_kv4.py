@@ -582,6 +582,49 @@ def test_calls_follow_one_another(rows, start, wait):
     assert _status() in (0, 8)          # some of them are written back, beyond the format
 
 
+@pytest.mark.parametrize("rows,start", [(1, 300), (1, 9000), (200, 900)])
+def test_captured_after_copies_fills_and_other_streams(rows, start):
+    """A graph in which a copy, a fill and a second stream's work come before
+    the calls, replayed with new rows."""
+    from kvp import kv4
+    gen = torch.Generator(device="cuda").manual_seed(rows + start)
+    x = torch.randn(3, rows, 256, device="cuda", generator=gen).to(BF)
+    pages, src = kv4.alloc_pages(80, 2).fill_(0x77), x[0].clone()
+    k, back = torch.zeros_like(src), torch.zeros_like(src)
+    q, out = torch.zeros(rows, 512, dtype=BF, device="cuda"), torch.zeros(rows, 512, dtype=BF, device="cuda")
+    other = torch.cuda.Stream()
+
+    def calls():
+        k.copy_(src)
+        kv4.write(pages, k, k, start=start)
+        here = torch.cuda.current_stream()
+        other.wait_stream(here)
+        with torch.cuda.stream(other):
+            q[:, :256].copy_(src)
+            kv4.read(pages, back, None, start=start)
+        here.wait_stream(other)
+        out.zero_()
+        kv4.attn(q, pages, out, heads=4, start=start)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    for i in (1, 2):
+        src.copy_(x[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), back.clone()
+        calls()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], out) and torch.equal(got[1], back)
+        assert bool((back.float() - x[i].float()).abs().max() < 0.5) and bool(out.any())
+    assert _status() == 0
+
+
 def test_two_streams_at_once():
     from kvp import kv4
     rng = np.random.default_rng(16)
