@@ -34,15 +34,12 @@ PAGE_HEAD = 18432     # bytes of one head's share of a page
 BLOCK = 1152          # bytes of 8 rows of one head
 
 
-_modules = {}
-
-
 def _kv4():
-    if not _modules:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "cuda-kv-persistence_b200"))
-        from kvp import kv4
-        _modules["kv4"] = kv4
-    return _modules["kv4"]
+    root = str(Path(__file__).resolve().parents[1] / "cuda-kv-persistence_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from kvp import kv4
+    return kv4
 
 
 def _dev():
