@@ -471,8 +471,8 @@ __global__ void __launch_bounds__(256) attn_kv4_join_units_kernel(const Kv4Param
     __shared__ float4 part[8][32];
     const int unit = (int)blockIdx.x / P.join_ctas, cta = (int)blockIdx.x % P.join_ctas;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    cudaGridDependencySynchronize();                  // the partials are complete, starts and counts visible
     const Kv4Unit u = unit_of(P, unit / P.span.kv_heads);
-    cudaGridDependencySynchronize();
     if (u.pages == 0) return;
     const int chunk = P.ws_unit[0], page = P.ws_unit[1 + unit], c0 = page / chunk;
     const int splits = (page + u.pages - 1) / chunk - c0 + 1;
