@@ -33,7 +33,7 @@ def test_every_kernel_is_found():
         "kv4_read_kernel", "kv4_write_kernel"]
 
 
-@pytest.mark.parametrize("name,body", _kernels(), ids=lambda x: x if x.endswith("_kernel") else "body")
+@pytest.mark.parametrize("name,body", list(_kernels()), ids=lambda x: x if x.endswith("_kernel") else "body")
 def test_nothing_is_read_before_the_wait(name, body):
     before, wait, _ = body.partition("cudaGridDependencySynchronize()")
     assert wait
