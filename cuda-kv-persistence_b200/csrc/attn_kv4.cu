@@ -474,9 +474,9 @@ __global__ void __launch_bounds__(256) attn_kv4_join_units_kernel(const Kv4Param
     cudaGridDependencySynchronize();                  // the partials are complete, starts and counts visible
     const Kv4Unit u = unit_of(P, unit / P.span.kv_heads);
     if (u.pages == 0) return;
-    const int chunk = P.ws_unit[0], page = P.ws_unit[1 + unit], c0 = page / chunk;
-    const int splits = (page + u.pages - 1) / chunk - c0 + 1;
-    if (splits == 1) return;                          // its rows are finished
+    const Kv4Pieces in = kv4_pieces(P.ws_unit[0], P.ws_unit[1 + unit], u.pages, P.ctas);
+    const int c0 = in.first, splits = in.count;
+    if (splits <= 1) return;                          // its rows are finished (or were given up)
     const int rows = min(u.rows - u.r0, 256), h = unit % P.span.kv_heads;
     auto add = [&](int row, int first, int step, float4& acc) {
         return add_partials(
@@ -640,6 +640,7 @@ int launch_attn_kv4(const Kv4Span& s, const Kv4Attn& a, int* d_status, cudaStrea
                     std::min(rounds, share + (double)cost(units - 1)) > share + 6 + units / 20.0;
         if (P.chunked) {
             grid = sms;
+            P.ctas = sms;
             slots = 2 * 256 * grid;
             // eight CTAs an SM, at least sixteen a unit (few units are in many pieces)
             P.join_ctas = (int)std::max(16LL, std::min(128LL, 8 * sms / units));

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "kv4.h"
+#include "kv4_pieces.h"
 
 namespace kvp {
 
@@ -20,6 +21,7 @@ struct Kv4Params {
     int group, max_rows;     // query heads per K/V head; rows * group
     int tokens, row_tiles, splits;
     int cluster;             // the splits of a row tile are one cluster and join by themselves
+    int ctas;                // (chunked) CTAs of the launch
     int join_ctas;           // (chunked) CTAs of the join for a unit
     int chunked;             // (many rows) the CTAs share the list of all units' pages evenly: see Kv4Unit
     float scale_log2;        // log2(e) / sqrt(128)
