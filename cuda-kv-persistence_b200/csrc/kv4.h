@@ -13,6 +13,8 @@
 // (halves away from zero).  Rounding s moves max|x| / s to 7.4375 at most, so
 // no value is clipped.  fp32 rows are rounded to bf16 first.  NaN is stored
 // as 0 and |x| > 26880 = 7 * 3840 as that bound; both set KVP_STATUS_RANGE.
+// Bytes above 215 can stand in unwritten rows only: K's at their value, V's
+// as 215 (vscale2), in reads and in attention.
 //
 // Layout.  Pages of 128 rows, uint8 [n_pages][kv_heads][18432]; a head's
 // share of a page is 16 blocks of 8 rows, each 1152 bytes: K codes [8 rows]

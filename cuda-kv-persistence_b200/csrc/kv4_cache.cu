@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kThreads)
             if (v) {
                 c[1][i] = *reinterpret_cast<const uint32_t*>(it.blk + kKv4VCode + (word >> 1) * 64 + r * 8 +
                                                              (word & 1) * 4);
-                e[1][i] = it.blk[kKv4VScale + (word >> 1) * 8 + r];
+                e[1][i] = min((uint32_t)it.blk[kKv4VScale + (word >> 1) * 8 + r], (uint32_t)kKv4TopScale);
             }
         }
 #pragma unroll

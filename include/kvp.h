@@ -310,7 +310,9 @@ int kvp_session_run_frames_batched(void* s, int f0, int nframes, const float* sc
  * significant bits, max |x| / 7 rounded to nearest, and hold x / scale
  * rounded to an integer in [-7, 7], so a value comes back off by at most
  * half a scale.  A page's bytes may be anything before they are written:
- * every bit pattern stands for finite numbers.
+ * every bit pattern stands for finite numbers.  (A scale byte eeeee mmm is
+ * (1 + m/8) 2^(e - 15).  215 is the largest that is written; a V scale byte
+ * above it, which only an unwritten row can hold, counts as 215.)
  *
  * A call touches rows [start, start + count) of each of `batch` sequences;
  * row i of a sequence is position start + i, and its page is

@@ -75,7 +75,8 @@ def get(pages: np.ndarray, page_ids, which: str) -> np.ndarray:
     t = pages[np.asarray(page_ids)].reshape(len(page_ids), pages.shape[1], 16, BLOCK)
     at, bit, sc = (_TAB[which][..., i] for i in range(3))
     n = ((t[..., at] >> bit.astype(np.uint8)) & 15).astype(np.int64) - 8
-    x = n * SCALES[t[..., sc]]                           # [page, head, block, row, dim]
+    # [page, head, block, row, dim]; V's scale bytes count up to the largest that is written
+    x = n * SCALES[t[..., sc] if which == "k" else np.minimum(t[..., sc], TOP_BYTE)]
     return x.transpose(0, 2, 3, 1, 4).reshape(-1, pages.shape[1], HEAD)
 
 
