@@ -728,8 +728,10 @@ KVP_API int kvp_session_run_frames_batched(void* sp, int f0, int nframes, const 
 }
 
 // ----------------------------------------------------------- 4-bit K/V cache
-// Field meanings: include/kvp.h.  Nothing here reads what the kvtm_*
-// managers stage, so their queued copies are left alone.
+// Field meanings: include/kvp.h.  Staging copies queued by kvtm_* managers are
+// issued first, as before the other attention launches: rows that are written
+// may lie in a manager's arena, rows that are read may go where a queued copy
+// still has to read from.
 struct kvp_kv4_span {
     void* pages;
     const int* page_map;
@@ -769,7 +771,9 @@ KVP_API int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* st
     const kvp::Kv4Span S = span_of(*s);
     const kvp::Kv4Rows R{r->k, r->v, r->row_stride, r->batch_stride, r->elem_bytes};
     // Bad arguments are reported before any device state is touched.
-    const int rc = kvp::check_kv4_rows(S, R, true);
+    int rc = kvp::check_kv4_rows(S, R, true);
+    if (rc != kvp::KVP_OK) return rc;
+    rc = kvp::flush_all_managers();
     if (rc != kvp::KVP_OK) return rc;
     int* st = kvp::status_word();
     if (!st) return kvp::KVP_ERR_CUDA;
@@ -780,7 +784,9 @@ KVP_API int kvp_kv4_read(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* str
     if (!s || !r) return kvp::KVP_ERR_ARG;
     const kvp::Kv4Span S = span_of(*s);
     const kvp::Kv4Rows R{r->k, r->v, r->row_stride, r->batch_stride, r->elem_bytes};
-    const int rc = kvp::check_kv4_rows(S, R, false);
+    int rc = kvp::check_kv4_rows(S, R, false);
+    if (rc != kvp::KVP_OK) return rc;
+    rc = kvp::flush_all_managers();
     if (rc != kvp::KVP_OK) return rc;
     int* st = kvp::status_word();
     if (!st) return kvp::KVP_ERR_CUDA;
@@ -792,7 +798,9 @@ KVP_API int kvp_attn_kv4(const kvp_kv4_span* s, const kvp_kv4_attn* a, void* str
     const kvp::Kv4Span S = span_of(*s);
     const kvp::Kv4Attn A{a->q, a->out, a->q_row_stride, a->q_batch_stride, a->out_row_stride,
                          a->out_batch_stride, a->heads, a->tokens, a->window, a->sinks};
-    const int rc = kvp::check_kv4_attn(S, A);
+    int rc = kvp::check_kv4_attn(S, A);
+    if (rc != kvp::KVP_OK) return rc;
+    rc = kvp::flush_all_managers();
     if (rc != kvp::KVP_OK) return rc;
     int* st = kvp::status_word();
     if (!st) return kvp::KVP_ERR_CUDA;

@@ -8,7 +8,7 @@
  *
  * Staging calls (kvtm_arena_stage, kvtm_streaming_stage) queue their row
  * copies; the copies run as one gather kernel at the next kvtm_*_window,
- * kvtm_*_end, kvtm_flush or attention launch, stream-ordered before it
+ * kvtm_*_end, kvtm_flush, attention launch or kvp_kv4_* call, stream-ordered before it
  * (the reference issued two cudaMemcpyAsync per row on stream 0).
  */
 #ifndef KVP_KV_TILE_MANAGER_H

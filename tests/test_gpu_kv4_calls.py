@@ -45,3 +45,63 @@ def test_reads_and_attention_agree_on_any_bytes(rows):
         assert np.array_equal(v, O.get(host, range(4), "v")[100: 100 + rows].reshape(rows, 256))
         assert np.all(np.abs(got - v) <= np.abs(v) / 128)
     assert _status() == 0
+
+
+def _staged(seed):
+    """A manager with five queued rows of 2 x 256 floats: (manager, k, v, slots' sources)."""
+    from kvp.manager import KVTileManager
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    k, v = (torch.randn(50, 256, device="cuda", generator=gen) for _ in range(2))
+    m = KVTileManager(20 * 2048, 20 * 2048)
+    assert m.init() and m.arena_init(20 * 2048, 512)
+    m.arena_begin_step()
+    src = []
+    for r in (3, 4, 5, 40, 41):
+        ok, slot = m.arena_stage(k[r].data_ptr(), 1024, v[r].data_ptr(), 1024)
+        assert ok and slot == len(src)
+        src.append(r)
+    assert m.pending_copies() == 10
+    return m, k, v, src
+
+
+def test_queued_copies_of_the_managers_go_first():
+    """Staging calls queue their row copies up to the next launch: a write may
+    take its rows from the arena, a read may fill rows that a copy reads."""
+    import ctypes as C
+
+    from kvp import kv4
+    from kvp._lib import Kv4Attn, Kv4Rows, Kv4Span, lib
+    L = lib()
+    pages = kv4.alloc_pages(1, 2)
+    span = Kv4Span(pages.data_ptr(), 0, 0, 0, 1, 2, 1, 1, 0, 5)
+
+    m, k, v, src = _staged(1)
+    arena = m.arena_device_ptr()
+    rows = Kv4Rows(arena, arena + 1024, 512, 0, 4)
+    bad = Kv4Rows(arena, arena + 1024, 510, 0, 4)
+    assert L.kvp_kv4_write(C.byref(span), C.byref(bad), None) == -1 and m.pending_copies() == 10
+    assert L.kvp_kv4_write(C.byref(span), C.byref(rows), None) == 0 and m.pending_copies() == 0
+    back = [torch.empty(5, 256, device="cuda") for _ in range(2)]
+    kv4.read(pages, *back)
+    for t, x in zip(back, (k, v)):
+        want = O.values(*O.quantise(x[src].double().cpu().numpy().reshape(5, 2, 128))).reshape(5, 256)
+        assert np.array_equal(t.double().cpu().numpy(), want)
+    m.close()
+
+    m, k, v, src = _staged(2)
+    kept = k.clone()
+    kv4.read(pages, k[3:8], None)                    # over three of the rows to be copied
+    assert m.pending_copies() == 0 and not torch.equal(k, kept)
+    staged = Kv4Rows(m.arena_device_ptr(), m.arena_device_ptr() + 1024, 512, 0, 4)
+    assert L.kvp_kv4_write(C.byref(span), C.byref(staged), None) == 0
+    kv4.read(pages, back[0], None)
+    want = O.values(*O.quantise(kept[src].double().cpu().numpy().reshape(5, 2, 128))).reshape(5, 256)
+    assert np.array_equal(back[0].double().cpu().numpy(), want)
+    m.close()
+
+    m, k, v, src = _staged(3)
+    q = torch.zeros(5, 256, dtype=BF, device="cuda")
+    attn = Kv4Attn(q.data_ptr(), q.data_ptr(), 256, 0, 256, 0, 2, 1, 0, 0)
+    assert L.kvp_attn_kv4(C.byref(span), C.byref(attn), None) == 0 and m.pending_copies() == 0
+    m.close()
+    assert _status() == 0
