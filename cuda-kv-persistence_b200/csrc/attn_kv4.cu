@@ -118,9 +118,11 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
     const int h = (int)(x % (uint32_t)s.kv_heads), b = (int)(x / (uint32_t)s.kv_heads);
     int start, count;
     cudaGridDependencySynchronize();                  // what was queued before is complete and visible
-    // The join may be launched (it waits for the data).  Where there is none the
-    // next call's CTAs are not let in among these: 33.9 us became 38.7 at 16
-    // sequences of 8191 keys x 8 heads.
+    // What comes next, a join or the next call, may be launched (it waits for the
+    // data).  Not where the splits are clusters: the next call's CTAs between
+    // these made 38.7 us of 33.9 at 16 sequences of 8191 keys x 8 heads.  With one
+    // split, and so no join, it is as long either way (20 sequences of 4096 keys
+    // x 8 heads 36.7 us, 160 of 300 30.4; 31 keys x 8 heads 3.8, without 3.9).
     if (!P.cluster) cudaTriggerProgrammaticLaunchCompletion();
     if (!sequence(s, b, start, count)) {
         if (threadIdx.x == 0) atomicOr(P.status, KVP_STATUS_MAP);
