@@ -766,10 +766,16 @@ KVP_API long long kvp_kv4_page_bytes(int kv_heads) {
     return kv_heads > 0 ? (long long)kv_heads * kvp::kKv4PageHeadBytes : kvp::KVP_ERR_ARG;
 }
 
-KVP_API int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream) {
-    if (!s || !r) return kvp::KVP_ERR_ARG;
+KVP_API int kvp_kv4_write_kv(const kvp_kv4_span* s, const kvp_kv4_rows* k, const kvp_kv4_rows* v,
+                             void* stream) {
+    if (!s || !k || !v) return kvp::KVP_ERR_ARG;
+    if (k->elem_bytes != v->elem_bytes) {
+        kvp::set_error("kv4_write: k and v must agree in elem_bytes");
+        return kvp::KVP_ERR_ARG;
+    }
     const kvp::Kv4Span S = span_of(*s);
-    const kvp::Kv4Rows R{r->k, r->v, r->row_stride, r->batch_stride, r->elem_bytes};
+    const kvp::Kv4Rows R{k->k, v->v, k->row_stride, k->batch_stride, k->elem_bytes,
+                         v->row_stride, v->batch_stride};
     // Bad arguments are reported before any device state is touched.
     int rc = kvp::check_kv4_rows(S, R, true);
     if (rc != kvp::KVP_OK) return rc;
@@ -780,10 +786,15 @@ KVP_API int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* st
     return kvp::launch_kv4_write(S, R, st, (cudaStream_t)stream);
 }
 
+KVP_API int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream) {
+    return kvp_kv4_write_kv(s, r, r, stream);
+}
+
 KVP_API int kvp_kv4_read(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream) {
     if (!s || !r) return kvp::KVP_ERR_ARG;
     const kvp::Kv4Span S = span_of(*s);
-    const kvp::Kv4Rows R{r->k, r->v, r->row_stride, r->batch_stride, r->elem_bytes};
+    const kvp::Kv4Rows R{r->k, r->v, r->row_stride, r->batch_stride, r->elem_bytes,
+                         r->row_stride, r->batch_stride};
     int rc = kvp::check_kv4_rows(S, R, false);
     if (rc != kvp::KVP_OK) return rc;
     rc = kvp::flush_all_managers();

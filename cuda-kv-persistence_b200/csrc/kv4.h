@@ -64,6 +64,7 @@ struct Kv4Rows {
     void* v;
     long long row_stride, batch_stride;
     int elem_bytes;          // 2 bf16, 4 fp32
+    long long v_row_stride, v_batch_stride;   // V's; outputs have K's
 };
 
 struct Kv4Attn {

@@ -136,8 +136,7 @@ __device__ __forceinline__ uint32_t quantise16(uint32_t (&x)[8], uint32_t (&word
 
 template <class T>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
-    kv4_write_kernel(const Kv4Span s, T* k, T* v, long long row_stride, long long batch_stride, int blocks,
-                     long long items, int* status) {
+    kv4_write_kernel(const Kv4Span s, const Kv4Rows r, int blocks, long long items, int* status) {
     __shared__ __align__(16) uint8_t stage[sizeof(T) == 4 ? kThreads / 32 : 1][4096];
     const int lane = threadIdx.x & 31;
     const long long step = (long long)gridDim.x * (kThreads / 32);
@@ -145,7 +144,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
     for (long long w = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < items; w += step) {
         Item it;
         if (!item_of(s, w, blocks, lane, status, it) || !it.blk) continue;
-        const long long col = it.b * batch_stride + it.h * 128;
+        const T* k = static_cast<const T*>(r.k) + it.b * r.batch_stride + it.h * 128;
+        const T* v = static_cast<const T*>(r.v) + it.b * r.v_batch_stride + it.h * 128;
         const int first = it.pos0 - it.start;          // row index of the block's row 0 (may be < 0)
         const int g = lane >> 2, t = lane & 3;
         // K: this lane's row g, dims [32t, 32t + 32)
@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
             uint8_t* st = stage[threadIdx.x >> 5];
             __syncwarp();                              // (the block before has been read)
             float4 yk[kKv4BlockRows], yv[kKv4BlockRows];
-            fetch_rows(yk, k + col, row_stride, first, it.count, lane);
-            fetch_rows(yv, v + col, row_stride, first, it.count, lane);
+            fetch_rows(yk, k, r.row_stride, first, it.count, lane);
+            fetch_rows(yv, v, r.v_row_stride, first, it.count, lane);
             stage_rows(st, yk, lane);
             stage_rows(st + 2048, yv, lane);
             __syncwarp();
@@ -168,14 +168,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
             load16(st + 2048, 2 * t, 2 * g, va);
             load16(st + 2048, 2 * t + 1, 2 * g, vb);
         } else {
-            const T* kp = k + col + (first + g) * row_stride + 32 * t;
-            const T* vp = v + col + (first + 2 * t) * row_stride + 16 * g;
+            const T* kp = k + (first + g) * r.row_stride + 32 * t;
+            const T* vp = v + (first + 2 * t) * r.v_row_stride + 16 * g;
             if (on) {
                 load16(kp, ka);
                 load16(kp + 16, kb);
             }
             if (on0) load16(vp, va);
-            if (on1) load16(vp + row_stride, vb);
+            if (on1) load16(vp + r.v_row_stride, vb);
         }
         if (on) {
             uint32_t c0[2], c1[2];
@@ -225,9 +225,10 @@ struct Out<float> {
 
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-    kv4_read_kernel(const Kv4Span s, T* k, T* v, long long row_stride, long long batch_stride, int blocks,
-                    long long items, int* status) {
+    kv4_read_kernel(const Kv4Span s, const Kv4Rows rows, int blocks, long long items, int* status) {
     constexpr int kDims = Out<T>::kDims, kLanes = 128 / kDims, kRows = 32 / kLanes;   // lanes of a row, rows of a pass
+    T* const k = static_cast<T*>(rows.k);
+    T* const v = static_cast<T*>(rows.v);
     const int lane = threadIdx.x & 31;
     const int dim = lane % kLanes * kDims, word = dim / 8, part = dim % 8 / 4;
     const long long step = (long long)gridDim.x * (kThreads / 32);
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kThreads)
         Item it;
         if (!item_of(s, w, blocks, lane, status, it)) continue;
         const int first = it.pos0 - it.start;
-        const long long at0 = it.b * batch_stride + it.h * 128 + dim;
+        const long long at0 = it.b * rows.batch_stride + it.h * 128 + dim;
         // every load first: a page that is not in the pool reads as codes of 0
         uint32_t c[2][8 / kRows], e[2][8 / kRows];
 #pragma unroll
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int i = 0; i < 8 / kRows; ++i) {
             const int r = kRows * i + lane / kLanes;
             if (first + r < 0 || first + r >= it.count) continue;
-            const long long at = at0 + (first + r) * row_stride;
+            const long long at = at0 + (first + r) * rows.row_stride;
             if (k) Out<T>::store(k + at, c[0][i], part, scale2(e[0][i] * 0x00010001u));
             if (v) Out<T>::store(v + at, c[1][i], part, scale2(e[1][i] * 0x00010001u));
         }
@@ -306,9 +307,8 @@ bool apart(const Kv4Span& s, long long row_stride, long long batch_stride, long 
            row_stride >= (s.batch - 1) * batch_stride + len;
 }
 
-template <class Row>
 int launch(const Kv4Span& s, const Kv4Rows& r, int* status, cudaStream_t stream,
-           void (*kernel)(Kv4Span, Row*, Row*, long long, long long, int, long long, int*)) {
+           void (*kernel)(Kv4Span, Kv4Rows, int, long long, int*)) {
     // rows may begin anywhere in a block: the last row's block is
     // (start % 8 + rows - 1) / 8 blocks after the first
     const int lead = s.starts ? kKv4BlockRows - 1 : s.start % kKv4BlockRows;
@@ -318,8 +318,7 @@ int launch(const Kv4Span& s, const Kv4Rows& r, int* status, cudaStream_t stream,
     cudaLaunchAttribute early;
     const cudaLaunchConfig_t cfg =
         kv4_config((unsigned)(ctas < 0x7fffffffLL ? ctas : 0x7fffffffLL), kThreads, 0, &early, stream);
-    KVP_CUDA(cudaLaunchKernelEx(&cfg, kernel, s, static_cast<Row*>(r.k), static_cast<Row*>(r.v), r.row_stride,
-                                r.batch_stride, blocks, items, status));
+    KVP_CUDA(cudaLaunchKernelEx(&cfg, kernel, s, r, blocks, items, status));
     return KVP_OK;
 }
 
@@ -337,14 +336,16 @@ int check_kv4_rows(const Kv4Span& s, const Kv4Rows& r, bool write) {
         set_error("%s: no rows", who);
         return KVP_ERR_ARG;
     }
-    const long long per16 = 16 / r.elem_bytes;
+    const long long per16 = 16 / r.elem_bytes, len = s.kv_heads * 128LL;
     if (((uintptr_t)r.k | (uintptr_t)r.v) & 15 || r.row_stride % per16 || r.batch_stride % per16 ||
-        (s.rows > 1 && r.row_stride < s.kv_heads * 128LL) || (s.batch > 1 && r.batch_stride < 0)) {
+        r.v_row_stride % per16 || r.v_batch_stride % per16 ||
+        (s.rows > 1 && (r.row_stride < len || r.v_row_stride < len)) ||
+        (s.batch > 1 && (r.batch_stride < 0 || r.v_batch_stride < 0))) {
         set_error("%s: rows must be 16-byte aligned, strides too, and a row stride at least kv_heads * 128", who);
         return KVP_ERR_ARG;
     }
     if (!write && s.rows > 0 && s.batch > 0 &&
-        (r.k == r.v || !apart(s, r.row_stride, r.batch_stride, s.kv_heads * 128LL))) {
+        (r.k == r.v || !apart(s, r.row_stride, r.batch_stride, len))) {
         set_error("kv4_read: the output rows overlap");
         return KVP_ERR_ARG;
     }

@@ -174,6 +174,7 @@ SIGNATURES = {
                                      C.c_int, C.c_float, C.c_void_p]),
     "kvp_kv4_page_bytes": (C.c_longlong, [C.c_int]),
     "kvp_kv4_write": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kvp_kv4_write_kv": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "kvp_kv4_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "kvp_attn_kv4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "kvp_session_plan_stack": (C.c_int, [C.c_void_p, C.c_void_p]),

@@ -6,9 +6,10 @@ kv_heads, 18432] (``alloc_pages``), and an int32 page map [batch, pages] that
 gives each sequence's pages in order (None: sequence b owns pages b *
 (n_pages // batch) and up).  Rows are [batch, rows, heads * 128] or, for one
 sequence, [rows, heads * 128]; only their last dimension has to be
-contiguous, so slices of a fused QKV buffer work.  A call touches the rows
-[start, start + rows) of every sequence; ``starts`` (int32 device tensor
-[batch]) gives each sequence its own start, ``counts`` fewer rows.
+contiguous, so slices of a fused QKV buffer work, V beside a K of its own
+too.  A call touches the rows [start, start + rows) of every sequence;
+``starts`` (int32 device tensor [batch]) gives each sequence its own start,
+``counts`` fewer rows.
 
     pages = kv4.alloc_pages(n, kv_heads)
     kv4.write(pages, k, v, page_map=m, start=s)          # the new rows
@@ -119,26 +120,27 @@ def _args(pages, a, b, names: str, types, heads, page_map, start: int, starts, c
                       n_pages, kv_heads, batch, stride, start, rows), rs, bs, b_rs, b_bs
 
 
-def _call(fn, what, dev, stream, span, args):
+def _call(fn, what, dev, stream, *args):
     if dev == _current_device():
-        rc = fn(span, args, _raw_stream(dev) if stream is None else stream)
+        rc = fn(*args, _raw_stream(dev) if stream is None else stream)
     else:
         with torch.cuda.device(dev):
-            rc = fn(span, args, _raw_stream(dev) if stream is None else stream)
+            rc = fn(*args, _raw_stream(dev) if stream is None else stream)
     if rc < 0:
         check(rc, what)
 
 
 def _kv(pages, k, v, page_map, start, starts, counts):
+    """Checks; (device, packed span, packed rows, v's rows if their strides are others)."""
     some, other = (k, v) if k is not None else (v, None)
     if some is None:
         _bad("no rows")
     dev, span, rs, bs, v_rs, v_bs = _args(pages, some, other, "k and v", _ROW_TYPES, None, page_map, start, starts,
                                           counts)
-    if rs != v_rs or bs != v_bs:
-        _bad("k and v must agree in strides")
-    return dev, span, _ROWS(0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), rs, bs,
-                            some.element_size())
+    k_at, v_at, size = 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), some.element_size()
+    if other is not None and (rs != v_rs or bs != v_bs):
+        return dev, span, _ROWS(k_at, 0, rs, bs, size), _ROWS(0, v_at, v_rs, v_bs, size)
+    return dev, span, _ROWS(k_at, v_at, rs, bs, size), None
 
 
 def write(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=None,
@@ -146,15 +148,22 @@ def write(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=Non
     """Quantises rows k, v (bf16 or fp32) into the cache."""
     if k is None or v is None:
         _bad("write needs k and v")
-    dev, span, rows = _kv(pages, k, v, page_map, start, starts, counts)
-    _call(lib().kvp_kv4_write, "kvp_kv4_write", dev, stream, span, rows)
+    dev, span, rows, v_rows = _kv(pages, k, v, page_map, start, starts, counts)
+    if v_rows is None:
+        _call(lib().kvp_kv4_write, "kvp_kv4_write", dev, stream, span, rows)
+    else:
+        _call(lib().kvp_kv4_write_kv, "kvp_kv4_write_kv", dev, stream, span, rows, v_rows)
 
 
 def read(pages, k, v, *, page_map=None, start: int = 0, starts=None, counts=None,
          stream=None) -> None:
     """Fills k and v (bf16 or fp32; either may be None) with the rows' values."""
-    dev, span, rows = _kv(pages, k, v, page_map, start, starts, counts)
+    dev, span, rows, v_rows = _kv(pages, k, v, page_map, start, starts, counts)
+    if v_rows is not None and k.data_ptr() == v.data_ptr():
+        _bad("the output rows overlap")
     _call(lib().kvp_kv4_read, "kvp_kv4_read", dev, stream, span, rows)
+    if v_rows is not None:
+        _call(lib().kvp_kv4_read, "kvp_kv4_read", dev, stream, span, v_rows)
 
 
 def attn(q, pages, out, *, heads: int, page_map=None, start: int = 0, starts=None, counts=None,

@@ -363,9 +363,14 @@ long long kvp_kv4_page_bytes(int kv_heads);
 /* Quantises the rows into the cache.  NaN is stored as 0 and |x| > 26880 as
  * that bound; either sets status bit 3. */
 int kvp_kv4_write(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream);
+/* The same for K and V whose strides differ (V a slice of a fused projection,
+ * say, and K a tensor of its own): k as k->k and its strides describe it, v as
+ * v->v and its own do; their elem_bytes agree. */
+int kvp_kv4_write_kv(const kvp_kv4_span* s, const kvp_kv4_rows* k, const kvp_kv4_rows* v, void* stream);
 
 /* The values the rows stand for (exact in bf16 and fp32).  Output rows must
- * not overlap. */
+ * not overlap.  K and V of other strides are two calls, each with the other
+ * NULL. */
 int kvp_kv4_read(const kvp_kv4_span* s, const kvp_kv4_rows* r, void* stream);
 
 /* softmax(q K^T / sqrt(128)) V over the cache: query row i of a sequence, at

@@ -105,3 +105,35 @@ def test_queued_copies_of_the_managers_go_first():
     assert L.kvp_attn_kv4(C.byref(span), C.byref(attn), None) == 0 and m.pending_copies() == 0
     m.close()
     assert _status() == 0
+
+
+@pytest.mark.parametrize("batch,rows,start", [(1, 1, 5), (3, 1, 127), (1, 40, 3), (2, 150, 121)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_k_and_v_of_different_strides(batch, rows, start, dtype):
+    """K a tensor of its own (or with the sequences inside the rows), V a slice of a fused projection."""
+    from kvp import kv4
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    v = torch.randn(batch, rows, 768, device="cuda", generator=gen).to(dtype)[..., 512:]
+    own = torch.randn(batch, rows, 256, device="cuda", generator=gen).to(dtype)
+    inside = own.transpose(0, 1).contiguous().transpose(0, 1)
+    host = np.random.default_rng(rows).integers(0, 256, (3 * batch, 2, O.PAGE_HEAD), dtype=np.uint8)
+    want = torch.from_numpy(host).cuda()
+    kv4.write(want, own, v.contiguous(), start=start)
+    fused = torch.full((batch, rows, 768), 7.0, dtype=dtype, device="cuda")
+    for k in (own, inside):
+        got = torch.from_numpy(host).cuda()
+        kv4.write(got, k, v, start=start)
+        assert torch.equal(got, want)
+        swapped = torch.from_numpy(host).cuda()
+        kv4.write(want2 := torch.from_numpy(host).cuda(), v.contiguous(), own, start=start)
+        kv4.write(swapped, v, k, start=start)
+        assert torch.equal(swapped, want2)
+        back = torch.empty_like(k)
+        kv4.read(got, back, fused[..., 512:], start=start)
+        for t, w in ((back, "k"), (fused[..., 512:], "v")):
+            for b in range(batch):
+                ids = range(3 * b, 3 * b + 3)
+                ref = O.get(want.cpu().numpy(), ids, w)[start: start + rows].reshape(rows, 256)
+                assert np.array_equal(t[b].double().cpu().numpy(), ref)
+    assert bool((fused[..., :512] == 7).all())
+    assert _status() == 0
