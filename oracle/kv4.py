@@ -95,15 +95,16 @@ def attention(q, k, v, ok):
     """q [rows, heads, 128], k / v [keys, kv_heads, 128], ok bool [rows, keys]
     -> out [rows, heads, 128] and a bound on |kernel - out|.
 
-    The bound counts a kernel's roundings: every weight to 16 bits (bf16: 2^-8
-    of it; fp16 with the largest at 2^7 or above: 2^-11 of it, or half of its
-    smallest step of 2^-24, which is 2^-25 / 2^7 = 2^-32 of the largest and so of
-    the sum of the weights, for every key: 2^-32 sum |v|), the result to bf16 (2^-8), the scores' fp32 sums of 128 products (each
-    partial sum off by 2^-23 of the sum of magnitudes, so a weight by d =
+    The bound counts the kernels' roundings, each at most half a step.
+    Weights P to fp16, the largest of a row at 2^7 or above: 2^-11 of each, or
+    half of fp16's smallest step of 2^-24, which is 2^-25 / 2^7 = 2^-32 of the
+    largest and so of the sum of the weights, for every key: 2^-32 sum |v|.
+    These enter the numerator alone.  The scores' fp32 sums of 128 products
+    (each partial sum off by 2^-23 of the sum of magnitudes, so a weight by d =
     130 * 2^-23 * max sum |q k| / sqrt(128)), the exponent's argument and the
-    exponential itself (2^-21 (1 + max |score|)); the weights enter numerator and
-    denominator; the sums over keys 2^-23 each at most 2^9 deep.  (A weight's
-    rounding to bf16 enters the numerator alone.)"""
+    exponential itself (2^-21 (1 + max |score|)): numerator and denominator.  The
+    sums over keys: 2^-23 each, at most 2^9 deep.  V is exact.  The result to
+    bf16: 2^-8 of it, the errors before included."""
     q, k, v = (torch.as_tensor(np.asarray(x, np.float64)) for x in (q, k, v))
     ok = torch.as_tensor(ok)
     rows, heads = q.shape[:2]
@@ -124,6 +125,6 @@ def attention(q, k, v, ok):
         mag = mag.amax(-1, keepdim=True) if mag.shape[1] else torch.zeros(rows, 1, dtype=torch.float64)
         d = 130 * 2.0 ** -23 * mag + 2.0 ** -21 * (1 + mag)
         out[:, h] = o
-        floor = 2.0 ** -32 * (ok.double() @ vv.abs())
-        tol[:, h] = (2.0 ** -8 + 2 * d + 2.0 ** -14) * a * (1 + 2.0 ** -8) + 2.0 ** -8 * o.abs() + floor
+        before = (2.0 ** -11 + 2 * d + 2.0 ** -14) * a + 2.0 ** -32 * (ok.double() @ vv.abs())
+        tol[:, h] = (1 + 2.0 ** -8) * before + 2.0 ** -8 * o.abs()
     return out.numpy(), tol.numpy()
