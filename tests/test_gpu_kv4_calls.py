@@ -137,3 +137,59 @@ def test_k_and_v_of_different_strides(batch, rows, start, dtype):
                 assert np.array_equal(t[b].double().cpu().numpy(), ref)
     assert bool((fused[..., :512] == 7).all())
     assert _status() == 0
+
+
+@pytest.mark.parametrize("rows,start", [(1, 300), (1, 4000), (1, 9000), (12, 5000), (40, 900), (300, 700), (300, 9000)])
+@pytest.mark.parametrize("mode", ["queued", "paused", "captured"])
+def test_what_a_call_has_written_is_what_the_next_one_reads(rows, start, mode):
+    """Copies, writes, attention and reads back to back.  A row's key is four times
+    its query, 22 or more above any other score, so its output is its own value: off
+    by half a scale, max / 14 * 17 / 16 < 0.4, and bf16's rounding, if pages, starts and
+    queries are those of this iteration, and nowhere near if they are the last one's."""
+    from kvp import kv4
+    gen = torch.Generator(device="cuda").manual_seed(rows + start)
+    pages = kv4.alloc_pages(80, 2).random_(0, 256, generator=gen)
+    field = pages.view(80, 2, 16, O.BLOCK)
+    for a in (512, 1088):
+        field[..., a: a + 64] = torch.randint(96, 112, field[..., a: a + 64].shape, device="cuda", generator=gen)
+    x = torch.randn(12, rows, 256, device="cuda", generator=gen).to(BF)
+    src = x[0].clone()
+    k, v, back = (torch.zeros_like(src) for _ in range(3))
+    q, out = (torch.zeros(rows, 512, dtype=BF, device="cuda") for _ in range(2))
+    again = torch.zeros_like(q)
+    at = torch.full((1,), start, dtype=torch.int32, device="cuda")
+
+    def wide(t):                                       # K/V head h for query heads 2h and 2h + 1
+        return t.view(rows, 2, 1, 128).expand(rows, 2, 2, 128).reshape(rows, 512)
+
+    steps = [lambda: torch.mul(src, 4, out=k), lambda: v.copy_(src), lambda: q.copy_(wide(src)),
+             lambda: kv4.write(pages, k, v, starts=at), lambda: kv4.attn(q, pages, out, heads=4, starts=at),
+             lambda: kv4.read(pages, None, back, starts=at), lambda: kv4.attn(q, pages, again, heads=4, starts=at),
+             lambda: kv4.write(pages, v, k, starts=at),    # (another content, until the next iteration)
+             lambda: at.add_(1)]
+
+    def once():
+        for step in steps:
+            step()
+            if mode == "paused":
+                torch.cuda.synchronize()
+
+    if mode == "captured":
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            once()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            once()
+        torch.cuda.synchronize()
+    outs = []
+    for i in range(12):
+        src.copy_(x[i])
+        graph.replay() if mode == "captured" else once()
+        outs.append(torch.cat((out, again, back), 1))
+    got = torch.stack(outs).float()
+    want = torch.stack([torch.cat((wide(y), wide(y), y), 1) for y in x]).float()
+    assert bool(((got - want).abs() < 0.5).all())
+    assert float((got[1:] - got[:-1]).abs().amax((1, 2)).min()) > 2
+    assert _status() == 0
