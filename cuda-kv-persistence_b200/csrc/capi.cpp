@@ -37,6 +37,11 @@ int* status_word() {
         if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
         if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) return nullptr;
         words[dev] = p;
+        // With it the pool that splits take their workspaces from: neither can
+        // be made while a stream is captured, and which call splits is not for
+        // the caller to know.  (A failure here is that call's to report.)
+        cudaMemPool_t pool = nullptr;
+        if (workspace_pool(&pool) != cudaSuccess) (void)cudaGetLastError();
     }
     return words[dev];
 }

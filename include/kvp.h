@@ -325,7 +325,8 @@ int kvp_session_run_frames_batched(void* s, int f0, int nframes, const float* sc
  * bit 0 and is left alone, its outputs too; so are rows at and behind
  * its count.  A call queues its work on `stream` and does not wait for the
  * device; the buffers belong to the current device.  The first call on a
- * device allocates the status word: make it before any stream capture.
+ * device, whichever it is, allocates the status word and the workspaces' pool:
+ * make it before any stream capture.
  * Several calls may run at once, on one cache too unless they write rows that
  * another one touches. */
 typedef struct {

@@ -193,3 +193,34 @@ def test_what_a_call_has_written_is_what_the_next_one_reads(rows, start, mode):
     assert bool(((got - want).abs() < 0.5).all())
     assert float((got[1:] - got[:-1]).abs().amax((1, 2)).min()) > 2
     assert _status() == 0
+
+
+@pytest.mark.parametrize("rows,start", [(1, 300), (1, 1200), (1, 9000), (12, 9000), (40, 900), (300, 900), (300, 9000)])
+def test_the_first_attention_of_a_process_is_captured(rows, start):
+    """One call on a device comes before the first capture there; a write will do."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = f"""
+import sys
+sys.path.insert(0, {str(Path(__file__).resolve().parents[1] / 'cuda-kv-persistence_b200')!r})
+import torch
+from kvp import kv4
+from kvp.attention import read_status
+pages = kv4.alloc_pages(80, 2).fill_(0x69)
+x = torch.randn({rows}, 256, device="cuda", generator=torch.Generator("cuda").manual_seed(0)).to(torch.bfloat16)
+kv4.write(pages, x, x, start={start})
+torch.cuda.synchronize()
+out, back, ref = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(x)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    kv4.attn(x, pages, out, heads=2, start={start})
+    kv4.read(pages, back, None, start={start})
+graph.replay()
+kv4.attn(x, pages, ref, heads=2, start={start})
+torch.cuda.synchronize()
+assert torch.equal(out, ref) and bool(out.any()) and bool((back.float() - x.float()).abs().max() < 0.5)
+assert read_status() == 0
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
