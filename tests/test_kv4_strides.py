@@ -64,3 +64,28 @@ def test_what_is_passed_on(calls, dtype):
     del seen[:]
     kv4.write(pages, k[:1, :1], v[:1, :1])
     assert [w for w, _ in seen] == ["kvp_kv4_write"]
+
+
+@pytest.mark.parametrize("stream", [None, 77])
+def test_a_call_on_another_device_than_the_current_one(monkeypatch, stream):
+    """The device is made current for the call, and its current stream is the call's."""
+    from kvp import kv4
+    log = []
+
+    class Device:
+        def __init__(self, d): self.d = d
+        def __enter__(self): log.append(("enter", self.d))
+        def __exit__(self, *a): log.append(("exit", self.d))
+
+    monkeypatch.setattr(kv4, "_current_device", lambda: 0)
+    monkeypatch.setattr(kv4, "_raw_stream", lambda dev: 1000 + dev)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    fn = lambda *a: log.append(a) or 0
+    kv4._call(fn, "kvp_kv4_write", 1, stream, b"span", b"rows")
+    assert log == [("enter", 1), (b"span", b"rows", 1001 if stream is None else stream), ("exit", 1)]
+    del log[:]
+    kv4._call(fn, "kvp_kv4_write", 0, stream, b"span", b"rows")
+    assert log == [(b"span", b"rows", 1000 if stream is None else stream)]
+    with pytest.raises(RuntimeError):                # (KvpError; other tests reload the module that defines it)
+        kv4._call(lambda *a: -1, "kvp_kv4_write", 1, stream, b"span", b"rows")
+    assert log[-1] == ("exit", 1)
