@@ -224,3 +224,39 @@ assert read_status() == 0
 """
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_calls_at_once_on_neighbouring_rows(dtype):
+    """Writes that run at once may share a block of eight rows, and reads and attention
+    go on beside them on rows that they do not touch."""
+    from kvp import kv4
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    cuts = [0, 13, 14, 15, 40, 41, 122, 131, 256, 259, 300]
+    x = torch.randn(2, 300, 256, device="cuda", generator=gen).to(dtype)
+    host = np.random.default_rng(1).integers(0, 256, (3, 2, O.PAGE_HEAD), dtype=np.uint8)
+    want = torch.from_numpy(host).cuda()
+    kv4.write(want, x[0], x[1])
+    q = torch.randn(5, 256, device="cuda", generator=gen).to(BF)
+    ref, k = torch.empty_like(q), torch.empty(84, 256, dtype=dtype, device="cuda")
+    kv4.attn(q, want, ref, heads=2, start=295)
+    got = torch.from_numpy(host).cuda()
+    streams = [torch.cuda.Stream() for _ in cuts[1:]]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got.copy_(torch.from_numpy(host))
+        torch.cuda.synchronize()
+        for s, a, b in zip(streams, cuts, cuts[1:]):
+            kv4.write(got, x[0, a:b], x[1, a:b], start=a, stream=s.cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        outs = [torch.empty_like(q) for _ in streams]
+        kv4.write(got, x[0, 10:12], x[1, 10:12], start=10, stream=streams[0].cuda_stream)    # as they are
+        kv4.read(got, k, None, start=300, stream=streams[1].cuda_stream)
+        for s, o in zip(streams[2:], outs[2:]):
+            kv4.attn(q, got, o, heads=2, start=295, window=200, stream=s.cuda_stream)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, outs[2]) for o in outs[2:])
+    kv4.attn(q, got, outs[0], heads=2, start=295)
+    assert torch.equal(outs[0], ref)
+    assert _status() == 0
