@@ -23,7 +23,7 @@ using namespace kv4_dev;
 using ptx::pack_f16;
 
 // ------------------------------------------------- few query rows: mma.sync
-// Bound by the cache's bytes: 144 a key and K/V head, against 2 * 128 * 2
+// Bound by the cache's bytes: 144 a key and K/V head, against 2 * 128
 // multiply-adds per query row.  Keys and dims go on the M side of
 // m16n8k16 and the query rows on the N side, so up to 8 rows cost the same:
 //   S^T[16 keys x 8] = K[16 x 128] Q^T,  O^T[16 dims x 8] += V^T[16 x 16] P^T.
@@ -33,12 +33,14 @@ using ptx::pack_f16;
 // straight from global memory, 512 consecutive bytes a warp, without shared
 // memory on the way; movmatrix turns P^T into the second product's operand.
 //
-// One query row over 32768 keys x 12 heads (56.6 MB) takes 19.9 us with its
-// join, 16 ragged sequences of up to 8191 keys x 8 heads 33.7 (3.4 TB/s),
-// 131072 keys x 12 heads 53.0 (4.3 TB/s).  The copies alone would take 41 of
-// those 53: turning codes into operands is about 530 instructions' issue
+// One query row over 32768 keys x 12 heads (56.6 MB) takes 20.1 us with its
+// join, 131072 keys x 12 heads 52.9 (4.3 TB/s).  The copies alone would take 41
+// of those 53: turning codes into operands is about 530 instructions' issue
 // cycles of the 1000 that a step of 32 keys takes, and the exponentials'
 // latency, which the warps of a scheduler reach together, most of the rest.
+// 16 ragged sequences of up to 8191 keys x 8 heads take 33.8 (3.4 TB/s): two
+// splits each, the longest of 4096 keys where an even share of what runs at
+// once is 2712.
 // K and V through a ring in shared memory, four warps a CTA, the next step's
 // first product between this one's exponentials and second: all measured
 // 0 to 6 % slower.
@@ -188,8 +190,8 @@ __global__ void __launch_bounds__(kDecThreads, NB == 1 ? 2 : 1) attn_kv4_rows_ke
 
     // A warp takes every eighth step of the CTA's range.  The next step's K
     // is on its way from the moment the current K is used up, its V likewise,
-    // and the page number after that one step longer: 9 KB a warp in flight
-    // at no registers beyond one step's.
+    // and the page number after that one step longer: up to one step's 4.6 KB
+    // a warp in flight, in that step's registers.
     bool any_bad = false;
     int u = u0 + warp, page = lookup(u), next = lookup(u + kWarps);
     if (u < u1) {

@@ -22,8 +22,8 @@
 //
 // One frame of 1560 rows over 32760 keys x 12 heads takes 344 us (913 TFLOP/s
 // of products that are needed, 55 % of what a large bf16 GEMM reaches), three
-// frames with a window of six and the first one kept 366, a token-causal
-// prompt of 4097 rows x 24 heads on 8 with a window of 1024 94.6.  A page takes a
+// frames with a window of six and the first one kept 367, a token-causal
+// prompt of 4097 rows x 24 heads on 8 with a window of 1024 94.1.  A page takes a
 // CTA about 3500 cycles, 2048 of them MMAs: a query tile's S, its exponentials
 // (1500; 1310 alone, 1024 of them MUFU's) and its PV follow one another, and
 // what lies between them counts: 240 cycles before the exponentials, 280 from

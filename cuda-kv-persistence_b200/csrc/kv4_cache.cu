@@ -5,8 +5,10 @@
 // which is what a scale's 16 dims and a page's blocks both divide into, so no
 // two warps share a byte; consecutive warps take consecutive heads of the same
 // rows, so a CTA's global rows are contiguous.  At 32760 bf16 rows x 12 heads
-// (258 MB) a write takes 44.9 us and a read 47.1, 5.7 and 5.5 TB/s; one
-// frame's write (1560 rows) 4.2 us and a token's 2.9, which is a launch.
+// (258 MB) a write takes 45.7 us and a read 44.1, 5.6 and 5.8 TB/s; one
+// frame's write (1560 rows) 4.0 us and a token's 2.4, which is a launch.  fp32:
+// 9000 rows x 8 heads (84 MB) in 21.7 us, 3.9 TB/s (a warp's loads, staging and
+// conversion follow one another, two CTAs of 117 registers an SM), out in 14.6, 5.8.
 #include "kernels.h"
 #include "kv4.h"
 
