@@ -326,7 +326,8 @@ int kvp_session_run_frames_batched(void* s, int f0, int nframes, const float* sc
  * its count.  A call queues its work on `stream` and does not wait for the
  * device; the buffers belong to the current device.  The first call on a
  * device, whichever it is, allocates the status word and the workspaces' pool:
- * make it before any stream capture.
+ * make it before any stream capture.  Queued kvtm_* staging copies are issued
+ * first, which a capture does not allow: kvtm_flush them before it.
  * Several calls may run at once, on one cache too unless they write rows that
  * another one touches. */
 typedef struct {
